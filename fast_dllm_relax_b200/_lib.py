@@ -46,6 +46,21 @@ class FdllmRequest(ctypes.Structure):
     ]
 
 
+class FdllmPagedCache(ctypes.Structure):
+    _fields_ = [
+        ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p),
+        ("layers", ctypes.c_int32), ("pages", ctypes.c_int32), ("page_size", ctypes.c_int32),
+    ]
+
+
+class FdllmPagedPlan(ctypes.Structure):
+    _fields_ = [
+        ("words", ctypes.c_int32), ("n", ctypes.c_int32), ("total_rows", ctypes.c_int32),
+        ("page_size", ctypes.c_int32), ("causal_block", ctypes.c_int32), ("table_cols", ctypes.c_int32),
+        ("max_position", ctypes.c_int32), ("priv", ctypes.c_int32 * 17),
+    ]
+
+
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 SIGNATURES: dict[str, tuple] = {
@@ -77,6 +92,12 @@ SIGNATURES: dict[str, tuple] = {
     "fdllm_device_error_detail": (_I, [_P, _P]),
     "fdllm_wait_selftest": (_I, [_P, ctypes.c_ulonglong, ctypes.POINTER(_I)]),
     "fdllm_workspace_bytes": (ctypes.c_longlong, [_P]),
+    "fdllm_paged_plan_batch": (_I, [_P, _P, _P, _P, _I, _I, _I, _P, _I, ctypes.POINTER(FdllmPagedPlan)]),
+    "fdllm_paged_append": (_I, [_P, ctypes.POINTER(FdllmPagedCache), _I, ctypes.POINTER(FdllmPagedPlan), _P, _P, _I,
+                                _P, _I, _P, _I, _P, _I, _P, _P, _I, _P, _P]),
+    "fdllm_paged_attention": (_I, [_P, ctypes.POINTER(FdllmPagedCache), _I, ctypes.POINTER(FdllmPagedPlan), _P, _P, _I,
+                                   _P, _I, ctypes.c_float, _P, _P]),
+    "fdllm_logprobs": (_I, [_P, _P, _I, _I, _I, ctypes.c_longlong, _P, _I, _P, _P, _P, _P, _P]),
 }
 
 _lib = None

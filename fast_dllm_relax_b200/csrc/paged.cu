@@ -1,0 +1,243 @@
+// Host side of the paged 8-bit KV cache and of the log-probability reduction: batch plans, argument
+// checks and the C ABI entries of include/fdllm_sm100.h.
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+#include <exception>
+#include <mutex>
+#include <string>
+#include <vector>
+
+#include "handle.h"
+#include "paged.h"
+
+using namespace fdllm;
+
+namespace {
+
+// No C++ exception crosses the ABI: `body` returns a status, an exception becomes one.
+template <typename F>
+int guarded(F body) {
+  try {
+    return body();
+  } catch (const std::exception& e) {
+    return fail(FDLLM_ERR_INVALID, std::string("internal error: ") + e.what());
+  } catch (...) {
+    return fail(FDLLM_ERR_INVALID, "internal error");
+  }
+}
+
+bool page_size_ok(int p) { return p == 16 || p == 32 || p == 64 || p == 128; }
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// Rows of `cols` elements with a row stride of ld elements, every row 16-byte aligned.
+int check_rows(const fdllm_handle* h, const char* name, const void* p, int ld, int cols) {
+  if (p == nullptr) return fail(FDLLM_ERR_INVALID, std::string(name) + ": null pointer");
+  if (ld < cols) return fail(FDLLM_ERR_INVALID, std::string(name) + ": row stride below " + std::to_string(cols));
+  if (!aligned16(p) || (static_cast<size_t>(ld) * h->esz) % 16 != 0)
+    return fail(FDLLM_ERR_INVALID, std::string(name) + ": rows must be 16-byte aligned");
+  return FDLLM_OK;
+}
+
+// The checks that append and attention share; *layer_codes / *layer_scales: this layer's offsets.
+int check_paged(const fdllm_handle* h, const fdllm_paged_cache* c, int layer, const fdllm_paged_plan* p,
+                const int32_t* words, const int32_t* table, int table_ld, size_t* layer_codes, size_t* layer_scales) {
+  if (c == nullptr || p == nullptr) return fail(FDLLM_ERR_INVALID, "null cache or plan");
+  if (c->k == nullptr || c->v == nullptr || c->k_scale == nullptr || c->v_scale == nullptr)
+    return fail(FDLLM_ERR_INVALID, "null paged cache");
+  if (!aligned16(c->k) || !aligned16(c->v)) return fail(FDLLM_ERR_INVALID, "paged cache must be 16-byte aligned");
+  if (c->layers <= 0 || c->pages <= 0 || !page_size_ok(c->page_size))
+    return fail(FDLLM_ERR_INVALID, "paged cache needs layers, pages and a page size of 16, 32, 64 or 128");
+  if (layer < 0 || layer >= c->layers)
+    return fail(FDLLM_ERR_INVALID, "layer " + std::to_string(layer) + " outside [0, " + std::to_string(c->layers) + ")");
+  if (p->page_size != c->page_size)
+    return fail(FDLLM_ERR_INVALID, "the plan is for pages of " + std::to_string(p->page_size) + " rows, the cache has " +
+                                       std::to_string(c->page_size));
+  if (p->total_rows > 0 && (words == nullptr || table == nullptr)) return fail(FDLLM_ERR_INVALID, "null plan words or table");
+  if (table_ld < p->table_cols)
+    return fail(FDLLM_ERR_INVALID, "page table has " + std::to_string(table_ld) + " columns; the longest request needs " +
+                                       std::to_string(p->table_cols));
+  const size_t heads = static_cast<size_t>(c->pages) * h->cfg.num_key_value_heads;
+  *layer_scales = static_cast<size_t>(layer) * heads;
+  *layer_codes = static_cast<size_t>(layer) * heads * c->page_size * h->cfg.head_dim;
+  return FDLLM_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int fdllm_paged_plan_batch(fdllm_handle* h, const int32_t* rows, const int32_t* start, const int32_t* live, int n,
+                           int page_size, int causal_block, int32_t* words, int cap, fdllm_paged_plan* plan) {
+  return guarded([&]() -> int {
+    if (h == nullptr) return fail(FDLLM_ERR_INVALID, "null handle");
+    if (plan == nullptr || n < 0 || (n > 0 && (rows == nullptr || start == nullptr)) || cap < 0 ||
+        (cap > 0 && words == nullptr))
+      return fail(FDLLM_ERR_INVALID, "bad plan arguments");
+    if (!page_size_ok(page_size)) return fail(FDLLM_ERR_INVALID, "page size must be 16, 32, 64 or 128");
+    if (causal_block < 0) return fail(FDLLM_ERR_INVALID, "causal_block must not be negative");
+    std::vector<PagedReq> reqs(n);
+    std::vector<PagedPageUnit> units;
+    long long total = 0, max_len = 0, max_pos = 0;
+    for (int i = 0; i < n; ++i) {
+      const long long r = rows[i], s = start[i], lv = live != nullptr ? live[i] : start[i];
+      if (r < 0 || s < 0 || lv < s)
+        return fail(FDLLM_ERR_INVALID, "request " + std::to_string(i) + ": rows and start must not be negative, and live (" +
+                                           std::to_string(lv) + ") not below start (" + std::to_string(s) + ")");
+      const long long len = std::max(lv, s + r);
+      if (len > (1LL << 30) || total + r > (1LL << 30)) return fail(FDLLM_ERR_INVALID, "batch too long");
+      reqs[i] = PagedReq{static_cast<int>(total), static_cast<int>(r), static_cast<int>(s), static_cast<int>(lv),
+                         static_cast<int>(len), {0, 0, 0}};
+      total += r;
+      max_len = std::max(max_len, len);
+      if (r > 0) max_pos = std::max(max_pos, s + r);
+      for (long long p = s / page_size; r > 0 && p <= (s + r - 1) / page_size; ++p)
+        units.push_back(PagedPageUnit{i, static_cast<int>(p)});
+    }
+    fdllm_paged_plan out{};
+    out.n = n;
+    out.total_rows = static_cast<int>(total);
+    out.page_size = page_size;
+    out.causal_block = causal_block;
+    out.table_cols = static_cast<int>((max_len + page_size - 1) / page_size);
+    out.max_position = static_cast<int>(max_pos);
+    int at = n * kPagedReqWords;
+    out.priv[kPagedPageUnits] = static_cast<int>(units.size());
+    out.priv[kPagedPageOff] = at;
+    at += 2 * static_cast<int>(units.size());
+    out.words = at;
+    *plan = out;
+    if (cap < at) {
+      if (cap == 0 && words == nullptr) return FDLLM_OK;  // size query
+      return fail(FDLLM_ERR_INVALID, "plan needs " + std::to_string(at) + " words, given " + std::to_string(cap));
+    }
+    if (n > 0) std::memcpy(words, reqs.data(), reqs.size() * sizeof(PagedReq));
+    if (!units.empty())
+      std::memcpy(words + out.priv[kPagedPageOff], units.data(), units.size() * sizeof(PagedPageUnit));
+    return FDLLM_OK;
+  });
+}
+
+int fdllm_paged_append(fdllm_handle* h, const fdllm_paged_cache* cache, int layer, const fdllm_paged_plan* plan,
+                       const int32_t* plan_words, const int32_t* table, int table_ld, const void* q, int ldq,
+                       const void* k, int ldk, const void* v, int ldv, const float* rope_cos, const float* rope_sin,
+                       int rope_rows, void* q_out, void* stream) {
+  return guarded([&]() -> int {
+    FDLLM_TRY(check_handle(h));
+    size_t codes, scales;
+    FDLLM_TRY(check_paged(h, cache, layer, plan, plan_words, table, table_ld, &codes, &scales));
+    if ((rope_cos == nullptr) != (rope_sin == nullptr)) return fail(FDLLM_ERR_INVALID, "rope_cos and rope_sin go together");
+    const int have = rope_cos != nullptr ? rope_rows : h->cfg.max_positions;
+    if (plan->max_position > have)
+      return fail(FDLLM_ERR_INVALID, "RoPE positions reach " + std::to_string(plan->max_position) + "; the tables have " +
+                                         std::to_string(have) + " rows");
+    if (rope_cos != nullptr && (!aligned16(rope_cos) || !aligned16(rope_sin)))
+      return fail(FDLLM_ERR_INVALID, "RoPE tables must be 16-byte aligned");
+    if (plan->total_rows == 0) return FDLLM_OK;
+    const fdllm_config& c = h->cfg;
+    if ((q == nullptr) != (q_out == nullptr)) return fail(FDLLM_ERR_INVALID, "q and q_out go together");
+    if (q != nullptr) {
+      FDLLM_TRY(check_rows(h, "q", q, ldq, c.num_attention_heads * c.head_dim));
+      FDLLM_TRY(check_rows(h, "q_out", q_out, c.num_attention_heads * c.head_dim, c.num_attention_heads * c.head_dim));
+    }
+    FDLLM_TRY(check_rows(h, "k", k, ldk, c.num_key_value_heads * c.head_dim));
+    FDLLM_TRY(check_rows(h, "v", v, ldv, c.num_key_value_heads * c.head_dim));
+    PagedAppendArgs a{};
+    a.reqs = reinterpret_cast<const PagedReq*>(plan_words);
+    a.units = reinterpret_cast<const PagedPageUnit*>(plan_words + plan->priv[kPagedPageOff]);
+    a.n_units = plan->priv[kPagedPageUnits];
+    a.n = plan->n;
+    a.total_rows = plan->total_rows;
+    a.table = table;
+    a.table_ld = table_ld;
+    a.k = static_cast<uint8_t*>(cache->k) + codes;
+    a.v = static_cast<uint8_t*>(cache->v) + codes;
+    a.k_scale = cache->k_scale + scales;
+    a.v_scale = cache->v_scale + scales;
+    a.pages = cache->pages;
+    a.page_size = cache->page_size;
+    a.hq = c.num_attention_heads;
+    a.hkv = c.num_key_value_heads;
+    a.hd = c.head_dim;
+    a.q_in = q;
+    a.k_in = k;
+    a.v_in = v;
+    a.ldq = ldq;
+    a.ldk = ldk;
+    a.ldv = ldv;
+    a.table_f32 = rope_cos != nullptr || h->dtype == FDLLM_FLOAT32;
+    a.cos = rope_cos != nullptr ? static_cast<const void*>(rope_cos) : h->rope_cos.p;
+    a.sin = rope_sin != nullptr ? static_cast<const void*>(rope_sin) : h->rope_sin.p;
+    a.q_out = q_out;
+    std::lock_guard<std::mutex> lock(h->mu);
+    a.err = h->err.p;
+    CUDA_TRY(launch_paged_append(a, h->dtype, static_cast<cudaStream_t>(stream)));
+    return FDLLM_OK;
+  });
+}
+
+int fdllm_paged_attention(fdllm_handle* h, const fdllm_paged_cache* cache, int layer, const fdllm_paged_plan* plan,
+                          const int32_t* plan_words, const int32_t* table, int table_ld, const void* q, int ldq,
+                          float scale, void* out, void* stream) {
+  return guarded([&]() -> int {
+    FDLLM_TRY(check_handle(h));
+    size_t codes, scales;
+    FDLLM_TRY(check_paged(h, cache, layer, plan, plan_words, table, table_ld, &codes, &scales));
+    if (!std::isfinite(scale)) return fail(FDLLM_ERR_INVALID, "scale must be finite");
+    if (plan->total_rows == 0) return FDLLM_OK;
+    const fdllm_config& c = h->cfg;
+    const int cols = c.num_attention_heads * c.head_dim;
+    FDLLM_TRY(check_rows(h, "q", q, ldq, cols));
+    FDLLM_TRY(check_rows(h, "out", out, cols, cols));
+    PagedAttnArgs a{};
+    a.reqs = reinterpret_cast<const PagedReq*>(plan_words);
+    a.n = plan->n;
+    a.total_rows = plan->total_rows;
+    a.table = table;
+    a.table_ld = table_ld;
+    a.k = static_cast<const uint8_t*>(cache->k) + codes;
+    a.v = static_cast<const uint8_t*>(cache->v) + codes;
+    a.k_scale = cache->k_scale + scales;
+    a.v_scale = cache->v_scale + scales;
+    a.pages = cache->pages;
+    a.page_size = cache->page_size;
+    a.hq = c.num_attention_heads;
+    a.hkv = c.num_key_value_heads;
+    a.hd = c.head_dim;
+    a.causal_block = plan->causal_block;
+    a.q = q;
+    a.ldq = ldq;
+    a.scale = scale;
+    a.out = out;
+    std::lock_guard<std::mutex> lock(h->mu);
+    a.err = h->err.p;
+    CUDA_TRY(launch_paged_attention_simt(a, h->dtype, static_cast<cudaStream_t>(stream)));
+    return FDLLM_OK;
+  });
+}
+
+int fdllm_logprobs(fdllm_handle* h, const void* logits, int logits_dtype, int rows, int vocab, long long ld,
+                   const int32_t* targets, int top, float* logprob, float* entropy, int32_t* top_ids,
+                   float* top_logprobs, void* stream) {
+  return guarded([&]() -> int {
+    FDLLM_TRY(check_handle(h));
+    if (logits_dtype != FDLLM_FLOAT32 && logits_dtype != FDLLM_BFLOAT16)
+      return fail(FDLLM_ERR_UNSUPPORTED, "logits must be fp32 or bf16");
+    if (rows < 0 || vocab <= 0) return fail(FDLLM_ERR_INVALID, "bad logits shape");
+    if (ld < vocab) return fail(FDLLM_ERR_INVALID, "logits row stride below the vocabulary");
+    if (top < 0 || top > kMaxTopLogprobs || top > vocab)
+      return fail(FDLLM_ERR_INVALID, "top must be in [0, " + std::to_string(std::min(kMaxTopLogprobs, vocab)) + "]");
+    if (rows == 0) return FDLLM_OK;
+    if ((targets == nullptr) != (logprob == nullptr)) return fail(FDLLM_ERR_INVALID, "targets and logprob go together");
+    if (top > 0 && (top_ids == nullptr || top_logprobs == nullptr)) return fail(FDLLM_ERR_INVALID, "null top outputs");
+    if (logits == nullptr) return fail(FDLLM_ERR_INVALID, "null logits");
+    LogprobArgs a{logits, rows, vocab, ld, targets, top, logprob, entropy, top_ids, top_logprobs, nullptr};
+    std::lock_guard<std::mutex> lock(h->mu);
+    a.err = h->err.p;
+    CUDA_TRY(launch_logprobs(a, logits_dtype, static_cast<cudaStream_t>(stream)));
+    return FDLLM_OK;
+  });
+}
+
+}  // extern "C"

@@ -1,0 +1,138 @@
+// Paged 8-bit KV cache: the plan's layout within its int32 words (built on the host by paged.cu,
+// read by the append and attention kernels) and the kernels' launch arguments.
+#pragma once
+
+#ifdef __CUDACC__
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+#endif
+#include "kernels.h"
+
+namespace fdllm {
+
+// One request of a plan: kPagedReqWords words at words[kPagedReqWords * i].
+constexpr int kPagedReqWords = 8;
+struct PagedReq {
+  int tok0;   // its first token row
+  int rows;   // its token rows
+  int start;  // cache position of its first token row
+  int live;   // cache rows that hold values before the call
+  int len;    // cached length the call attends: max(live, start + rows)
+  int pad[3];
+};
+static_assert(sizeof(PagedReq) == 4 * kPagedReqWords, "plan request layout");
+
+// One page that an append writes: words[page_off + 2 * u].
+struct PagedPageUnit {
+  int req;
+  int slot;  // page number within the request
+};
+
+// fdllm_paged_plan::priv
+enum PagedPriv : int {
+  kPagedPageUnits = 0,  // number of page units
+  kPagedPageOff = 1,    // word offset of the page units
+};
+
+struct PagedAppendArgs {
+  const PagedReq* reqs;
+  const PagedPageUnit* units;
+  int n_units, n, total_rows;
+  const int* table;
+  int table_ld;
+  uint8_t *k, *v;          // this layer's codes [pages, hkv, page_size, hd]
+  float *k_scale, *v_scale;  // this layer's scales [pages, hkv]
+  int pages, page_size;
+  int hq, hkv, hd;
+  const void *q_in, *k_in, *v_in;
+  int ldq, ldk, ldv;
+  const void *cos, *sin;   // fp32 tables, or the handle's in its dtype (table_f32 = 0)
+  int table_f32;
+  int rope_rows;
+  void* q_out;
+  int* err;
+};
+
+struct PagedAttnArgs {
+  const PagedReq* reqs;
+  int n, total_rows;
+  const int* table;
+  int table_ld;
+  const uint8_t *k, *v;
+  const float *k_scale, *v_scale;
+  int pages, page_size;
+  int hq, hkv, hd;
+  int causal_block;
+  const void* q;
+  int ldq;
+  float scale;
+  void* out;
+  int* err;
+};
+
+constexpr int kMaxTopLogprobs = 32;
+
+struct LogprobArgs {
+  const void* logits;
+  int rows, vocab;
+  long long ld;
+  const int* targets;
+  int top;
+  float *logprob, *entropy;
+  int* top_ids;
+  float* top_logprobs;
+  int* err;
+};
+
+int launch_paged_append(const PagedAppendArgs& a, int dtype, cudaStream_t s);
+int launch_paged_attention_simt(const PagedAttnArgs& a, int dtype, cudaStream_t s);
+int launch_logprobs(const LogprobArgs& a, int dtype, cudaStream_t s);
+
+#ifdef __CUDACC__
+// ---- float8 e4m3 (1 sign, 4 exponent, 3 mantissa bits; largest 448, no infinities) --------------
+__device__ __forceinline__ uint16_t e4m3x2_from_f32(float lo, float hi) {  // nearest even, saturating
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+__device__ __forceinline__ uint32_t f16x2_from_e4m3x2(uint16_t c) {  // exact
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(c));
+  return r;
+}
+
+__device__ __forceinline__ float2 f32x2_from_e4m3x2(uint16_t c) {
+  const uint32_t h = f16x2_from_e4m3x2(c);
+  return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+
+// The request that owns token row `tok`: the last one with tok0 <= tok (empty requests share the
+// tok0 of the next one, so the last is the owner).
+__device__ __forceinline__ int paged_req_of(const PagedReq* reqs, int n, int tok) {
+  int lo = 0, hi = n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (reqs[mid].tok0 <= tok) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+// Page id of a table entry, bounds-checked: outside [0, pages) records the error and gives -1.
+__device__ __forceinline__ int paged_page_id(int id, int pages, int* err) {
+  if (id >= 0 && id < pages) return id;
+  report_error(err, kErrCacheRange);
+  return -1;
+}
+
+// Cache rows the token row at position `pos` attends.
+__device__ __forceinline__ int paged_key_limit(int len, int pos, int causal_block) {
+  if (causal_block <= 0) return len;
+  const long long lim = (static_cast<long long>(pos / causal_block) + 1) * causal_block;
+  return lim < len ? static_cast<int>(lim) : len;
+}
+#endif
+
+}  // namespace fdllm

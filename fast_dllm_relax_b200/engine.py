@@ -22,6 +22,7 @@ import torch
 
 from . import _lib
 from .config import ModelConfig
+from .paged import PagedCache, PagedPlan
 
 _DT = {"float32": (torch.float32, 0), "bfloat16": (torch.bfloat16, 1)}
 
@@ -278,6 +279,108 @@ class Engine:
         _lib.check(self.lib.fdllm_token_logprob(self._h, h2.data_ptr(), n, tg.data_ptr(), out.data_ptr(), self._stream()))
         return out
 
+    def logprobs(self, logits: torch.Tensor, targets: torch.Tensor | None = None, top: int = 0):
+        """Log probabilities of given tokens, with entropy and top alternatives (fdllm_logprobs):
+        logits [rows, vocab] fp32 or bf16 (rows may be strided, as in logits[:, ::2] of a step),
+        targets [rows] ids or None.  Returns (logprob [rows] or None, entropy [rows] in nats, top_ids
+        int32 [rows, top], top_logprobs [rows, top]): the `top` (up to 32) largest in order, ties to
+        the lowest id."""
+        codes = {torch.float32: 0, torch.bfloat16: 1}
+        x = logits[0] if logits.dim() == 3 and logits.shape[0] == 1 else logits
+        if x.dim() != 2 or x.dtype not in codes or x.device != self.device:
+            raise ValueError(f"logprobs: expected fp32 or bf16 logits [rows, vocab] on {self.device}, got "
+                             f"{x.dtype} {tuple(x.shape)} on {x.device}")
+        n, vocab = x.shape
+        if (vocab > 1 and x.stride(1) != 1) or (n > 1 and x.stride(0) < vocab):
+            x = x.contiguous()
+        tg = lp = None
+        if targets is not None:
+            tg = targets.to(self.device, torch.int32).contiguous().reshape(-1)
+            if tg.numel() != n:
+                raise ValueError("logprobs: one target per row")
+            lp = torch.empty(n, dtype=torch.float32, device=self.device)
+        ent = torch.empty(n, dtype=torch.float32, device=self.device)
+        top = int(top)
+        ids = torch.empty((n, max(top, 0)), dtype=torch.int32, device=self.device)
+        tlp = torch.empty((n, max(top, 0)), dtype=torch.float32, device=self.device)
+        _lib.check(self.lib.fdllm_logprobs(self._h, x.data_ptr(), codes[x.dtype], n, vocab,
+                                           int(x.stride(0)) if n > 1 else vocab, _ptr(tg), top, _ptr(lp),
+                                           ent.data_ptr(), ids.data_ptr() if top > 0 else None,
+                                           tlp.data_ptr() if top > 0 else None, self._stream()))
+        return lp, ent, ids, tlp
+
+    # ---- paged 8-bit cache --------------------------------------------------------------------
+    def new_paged_cache(self, pages: int, page_size: int = 32, layers: int | None = None) -> PagedCache:
+        """An empty page pool for `layers` layers (all of the model's by default)."""
+        c = self.cfg
+        shape = (c.num_hidden_layers if layers is None else int(layers), int(pages), c.num_key_value_heads,
+                 int(page_size), c.head_dim)
+        codes = [torch.zeros(shape, dtype=torch.uint8, device=self.device).view(torch.float8_e4m3fn) for _ in range(2)]
+        scales = [torch.ones(shape[:3], dtype=torch.float32, device=self.device) for _ in range(2)]
+        return PagedCache(*codes, *scales)
+
+    def paged_plan(self, rows: Sequence[int], start: Sequence[int], live: Sequence[int] | None = None, *,
+                   page_size: int = 32, causal_block: int = 0) -> PagedPlan:
+        """Lay out a batch (fdllm_paged_plan_batch): rows[i] token rows of request i at cache positions
+        start[i].., live[i] cache rows held before the call (default start[i]).  causal_block 0: every
+        row attends its request's whole length; B > 0: block-causal in blocks of B positions."""
+        n = len(rows)
+        if len(start) != n or (live is not None and len(live) != n):
+            raise ValueError("paged_plan: one start (and live) per request")
+        arrays = [(ctypes.c_int32 * max(n, 1))(*[int(x) for x in a]) if a is not None else None
+                  for a in (rows, start, live)]
+        desc = _lib.FdllmPagedPlan()
+        args = (self._h, *arrays, n, int(page_size), int(causal_block))
+        _lib.check(self.lib.fdllm_paged_plan_batch(*args, None, 0, ctypes.byref(desc)))
+        staging = torch.empty(max(desc.words, 1), dtype=torch.int32, pin_memory=True)
+        _lib.check(self.lib.fdllm_paged_plan_batch(*args, staging.data_ptr(), staging.numel(), ctypes.byref(desc)))
+        return PagedPlan(desc, staging.to(self.device, non_blocking=True), staging)
+
+    def paged_append(self, cache: PagedCache, layer: int, plan: PagedPlan, table: torch.Tensor,
+                     q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor,
+                     rope: tuple[torch.Tensor, torch.Tensor] | None = None) -> torch.Tensor | None:
+        """Append the plan's token rows to `layer` of the cache, rotating queries and keys on the way
+        (fdllm_paged_append).  q [total_rows, heads * head_dim] (or None), k and v [total_rows, kv_heads *
+        head_dim] before RoPE; views of a packed qkv tensor are taken as they are.  table: int32
+        [n, columns] page ids.  rope: fp32 (cos, sin) tables [positions, head_dim / 2], else the
+        engine's.  Returns the rotated queries."""
+        c = self.cfg
+        pc = self._paged(cache, plan, table, "paged_append")
+        cols = (c.num_attention_heads * c.head_dim, c.num_key_value_heads * c.head_dim)
+        q = None if q is None else self._token_rows(q, plan, cols[0], "paged_append: q")
+        k, v = (self._token_rows(t, plan, cols[1], f"paged_append: {s}") for t, s in ((k, "k"), (v, "v")))
+        cos = sin = None
+        if rope is not None:
+            cos, sin = rope
+            for t in (cos, sin):
+                if t.device != self.device or t.dtype != torch.float32 or t.dim() != 2 or not t.is_contiguous() \
+                        or t.shape[1] != c.head_dim // 2 or t.shape != cos.shape:
+                    raise ValueError(f"paged_append: rope tables must be contiguous fp32 [positions, {c.head_dim // 2}] "
+                                     f"on {self.device}")
+        out = None if q is None else torch.empty((plan.total_rows, cols[0]), dtype=self.dtype, device=self.device)
+        _lib.check(self.lib.fdllm_paged_append(
+            self._h, ctypes.byref(pc), int(layer), ctypes.byref(plan.desc), plan.words.data_ptr(), table.data_ptr(),
+            int(table.shape[1]), _ptr(q), 0 if q is None else int(q.stride(0)), k.data_ptr(), int(k.stride(0)),
+            v.data_ptr(), int(v.stride(0)), _ptr(cos), _ptr(sin), 0 if cos is None else int(cos.shape[0]), _ptr(out),
+            self._stream()))
+        return out
+
+    def paged_attention(self, cache: PagedCache, layer: int, plan: PagedPlan, table: torch.Tensor, q: torch.Tensor,
+                        scale: float | None = None) -> torch.Tensor:
+        """Attention of the plan's token rows over `layer` of the cache (fdllm_paged_attention): q
+        [total_rows, heads * head_dim], rotated -> [total_rows, heads * head_dim].  scale defaults to
+        head_dim ** -0.5."""
+        c = self.cfg
+        pc = self._paged(cache, plan, table, "paged_attention")
+        cols = c.num_attention_heads * c.head_dim
+        q = self._token_rows(q, plan, cols, "paged_attention: q")
+        out = torch.empty((plan.total_rows, cols), dtype=self.dtype, device=self.device)
+        _lib.check(self.lib.fdllm_paged_attention(
+            self._h, ctypes.byref(pc), int(layer), ctypes.byref(plan.desc), plan.words.data_ptr(), table.data_ptr(),
+            int(table.shape[1]), q.data_ptr(), int(q.stride(0)), float(c.head_dim ** -0.5 if scale is None else scale),
+            out.data_ptr(), self._stream()))
+        return out
+
     def generate(self, prompt_ids: Sequence[int], *, max_new_tokens: int, block_size: int = 32,
                  small_block_size: int = 8, threshold: float = 0.9, use_block_cache: bool = False, mask_id: int,
                  stop_token: int | None = None, timing: dict | None = None) -> tuple[list[int], dict]:
@@ -350,6 +453,32 @@ class Engine:
         return int(self.lib.fdllm_workspace_bytes(self._h))
 
     # ---- argument normalisation --------------------------------------------------------------
+    def _paged(self, cache: PagedCache, plan: PagedPlan, table: torch.Tensor, name: str):
+        c = self.cfg
+        if cache.k.device != self.device or cache.k.shape[2] != c.num_key_value_heads or cache.k.shape[4] != c.head_dim:
+            raise ValueError(f"{name}: cache must be [layers, pages, {c.num_key_value_heads}, page_size, {c.head_dim}] on "
+                             f"{self.device}, got {tuple(cache.k.shape)} on {cache.k.device}")
+        if table.dim() != 2 or table.dtype != torch.int32 or table.device != self.device or not table.is_contiguous() \
+                or table.shape[0] != plan.desc.n:
+            raise ValueError(f"{name}: table must be a contiguous int32 [{plan.desc.n}, columns] tensor on {self.device}")
+        if plan.words.device != self.device:
+            raise ValueError(f"{name}: the plan is on {plan.words.device}")
+        return _lib.FdllmPagedCache(cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(),
+                                    cache.v_scale.data_ptr(), cache.layers, cache.pages, cache.page_size)
+
+    def _token_rows(self, t: torch.Tensor, plan: PagedPlan, cols: int, name: str) -> torch.Tensor:
+        """[total_rows, cols] in the engine's dtype with 16-byte aligned rows: strided views pass as they
+        are, others are copied."""
+        if t.device != self.device or t.dtype != self.dtype or t.dim() < 2 or t.shape[0] != plan.total_rows \
+                or t[:1].numel() != (cols if plan.total_rows else 0):
+            raise ValueError(f"{name}: expected {self.dtype} [{plan.total_rows}, {cols}] on {self.device}, got "
+                             f"{t.dtype} {tuple(t.shape)} on {t.device}")
+        t = t.reshape(plan.total_rows, cols)
+        unit = 16 // t.element_size()
+        if t.stride(1) != 1 or t.stride(0) < cols or t.stride(0) % unit or t.data_ptr() % 16:
+            t = t.contiguous() if not t.is_contiguous() else t.clone()
+        return t
+
     def _bias(self, bias: torch.Tensor | None, T: int) -> torch.Tensor | None:
         if bias is None:
             return None

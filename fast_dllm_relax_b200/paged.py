@@ -1,0 +1,71 @@
+"""Paged 8-bit KV caches: the page pool and the batch plan of `Engine.paged_append` and
+`Engine.paged_attention` (the reference's caches are one contiguous buffer per request).
+
+    cache = eng.new_paged_cache(pages, page_size=32)
+    plan = eng.paged_plan(rows, start, page_size=32)          # one per step, shared by every layer
+    q = eng.paged_append(cache, layer, plan, table, q, k, v)  # rotate, code, write
+    o = eng.paged_attention(cache, layer, plan, table, q)
+"""
+
+from __future__ import annotations
+
+import dataclasses
+
+import torch
+
+PAGE_SIZES = (16, 32, 64, 128)
+
+
+@dataclasses.dataclass
+class PagedCache:
+    """A pool of pages: float8 e4m3 codes [layers, pages, kv_heads, page_size, head_dim] of the keys
+    and of the values, and fp32 scales [layers, pages, kv_heads]; a cached value is code * scale."""
+
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scale: torch.Tensor
+    v_scale: torch.Tensor
+
+    def __post_init__(self):
+        if self.k.dim() != 5 or self.k.shape != self.v.shape:
+            raise ValueError("paged cache: k and v must be [layers, pages, kv_heads, page_size, head_dim]")
+        if self.k.shape[3] not in PAGE_SIZES:
+            raise ValueError(f"paged cache: page size must be one of {PAGE_SIZES}, got {self.k.shape[3]}")
+        for t in (self.k, self.v):
+            if t.dtype != torch.float8_e4m3fn or not t.is_contiguous():
+                raise ValueError("paged cache: codes must be contiguous float8_e4m3fn")
+        for t in (self.k_scale, self.v_scale):
+            if t.dtype != torch.float32 or not t.is_contiguous() or t.shape != self.k.shape[:3]:
+                raise ValueError("paged cache: scales must be contiguous float32 [layers, pages, kv_heads]")
+        if len({t.device for t in (self.k, self.v, self.k_scale, self.v_scale)}) != 1:
+            raise ValueError("paged cache: tensors on different devices")
+
+    @property
+    def layers(self) -> int:
+        return int(self.k.shape[0])
+
+    @property
+    def pages(self) -> int:
+        return int(self.k.shape[1])
+
+    @property
+    def page_size(self) -> int:
+        return int(self.k.shape[3])
+
+
+class PagedPlan:
+    """A laid-out batch (fdllm_paged_plan_batch): the host description and its words on the device.
+    `words` is read by the calls that take the plan, in stream order after its upload."""
+
+    def __init__(self, desc, words: torch.Tensor, staging: torch.Tensor):
+        self.desc = desc
+        self.words = words
+        self._staging = staging  # pinned source of the upload, alive as long as the plan
+
+    @property
+    def total_rows(self) -> int:
+        return int(self.desc.total_rows)
+
+    @property
+    def table_cols(self) -> int:
+        return int(self.desc.table_cols)

@@ -230,6 +230,94 @@ FDLLM_API int fdllm_kernel_trace_read(fdllm_handle* h, uint64_t* out, int32_t* k
 FDLLM_API int fdllm_confidence_static(fdllm_handle* h, const void* hidden, int rows, int32_t* ids, float* maxp,
                                       void* stream);
 
+/* ---- paged 8-bit KV cache -----------------------------------------------------------------------
+ * (no counterpart in the reference, whose caches are one contiguous buffer per request).
+ *
+ * A cache is a pool of pages.  A page holds page_size cache rows of one request: per layer and KV
+ * head, float8 e4m3 codes of the keys and of the values and one fp32 scale each; the value of a
+ * code is code * scale.  Cache row t of request r lives in page table[r][t / page_size], row
+ * t % page_size.  Half the bytes of a bf16 cache, no per-request capacity, nothing copied when a
+ * request grows. */
+typedef struct fdllm_paged_cache {
+  void* k;               /* e4m3 codes [layers, pages, kv_heads, page_size, head_dim], 16-byte aligned */
+  void* v;
+  float* k_scale;        /* fp32 [layers, pages, kv_heads], normal positive */
+  float* v_scale;
+  int32_t layers;
+  int32_t pages;
+  int32_t page_size;     /* 16, 32, 64 or 128 */
+} fdllm_paged_cache;
+
+/* A batch of requests over paged caches, laid out by fdllm_paged_plan for the kernels.  The caller
+ * copies the plan's `words` int32 words to device memory once and hands both to any number of
+ * append / attention calls (every layer of a step uses the same plan). */
+typedef struct fdllm_paged_plan {
+  int32_t words;         /* int32 words of the device copy */
+  int32_t n;             /* requests */
+  int32_t total_rows;    /* token rows of all requests, concatenated in request order */
+  int32_t page_size;
+  int32_t causal_block;
+  int32_t table_cols;    /* columns a page table needs: pages of the longest request */
+  int32_t max_position;  /* 1 + the largest position of a token row */
+  int32_t priv[17];      /* offsets and counts within the words (library-internal) */
+} fdllm_paged_plan;
+
+/* Lay out a batch.  Host arrays of n: rows[i] >= 0 token rows of request i at cache positions
+ * [start[i], start[i] + rows[i]); live[i] >= start[i] cache rows that hold values before the call
+ * (NULL: live = start, a plain append).  Its cached length is len = max(live, start + rows).
+ * causal_block 0: a token row attends all len cache rows (the bidirectional block of a cached
+ * forward); B > 0: the row at position p attends rows [0, min(len, (p / B + 1) * B)).
+ * words: host int32[cap], receives the plan's words; with cap too small the call returns
+ * FDLLM_ERR_INVALID with plan->words set (cap 0 and words NULL query the size). */
+FDLLM_API int fdllm_paged_plan_batch(fdllm_handle* h, const int32_t* rows, const int32_t* start, const int32_t* live,
+                                     int n, int page_size, int causal_block, int32_t* words, int cap,
+                                     fdllm_paged_plan* plan);
+
+/* Append the batch's token rows to the cache, with the position rotation applied on the way.
+ * q [total_rows, heads * head_dim], k and v [total_rows, kv_heads * head_dim], in the handle's
+ * dtype, before RoPE, each with its own row stride in elements (16-byte aligned rows; views of one
+ * packed qkv tensor work).  Row i of request r sits at position start[r] + i; its halves (x1, x2)
+ * of a head become (x1 cos - x2 sin, x2 cos + x1 sin) in fp32 with the tables' row at that position:
+ * rope_cos / rope_sin fp32 [rope_rows, head_dim / 2], or NULL for the handle's own tables.
+ * q_out [total_rows, heads * head_dim] (contiguous) receives the rotated queries (q and q_out NULL:
+ * no queries).  Rotated keys and the values are coded straight from fp32, one rounding:
+ *   scale of a touched page = the least power of two (>= 2^-64) that brings its new finite values
+ *   into +-448, or the page's present scale if that is larger and the page keeps rows;
+ *   code = e4m3(value / scale), nearest even; infinities saturate, NaN stays NaN.
+ * Rows of a touched page below `live` and outside the written range keep their values; when the
+ * scale grows their codes are rounded again to it (exact for e4m3 normal results).  Other rows of
+ * the page are not read or written.  table: device int32 [n, table_ld] page ids; an id outside
+ * [0, pages) writes nothing and records device error 6.  No page may be touched by two requests of
+ * the batch. */
+FDLLM_API int fdllm_paged_append(fdllm_handle* h, const fdllm_paged_cache* cache, int layer,
+                                 const fdllm_paged_plan* plan, const int32_t* plan_words, const int32_t* table,
+                                 int table_ld, const void* q, int ldq, const void* k, int ldk, const void* v, int ldv,
+                                 const float* rope_cos, const float* rope_sin, int rope_rows, void* q_out,
+                                 void* stream);
+
+/* Attention of the batch's token rows over the cache: q [total_rows, heads * head_dim] (rotated, row
+ * stride ldq elements, 16-byte aligned rows) -> out [total_rows, heads * head_dim] (contiguous),
+ *   out = sum_t softmax_t(scale * q . k_t) v_t   over the rows the plan's mask leaves,
+ * fp32 softmax and accumulation; a token row that attends nothing gets zeros.  Cache rows at or past
+ * a request's length are never used, whatever their bytes hold; rows below it must hold finite codes.
+ * A page id outside [0, pages) is read as page 0 and records device error 6. */
+FDLLM_API int fdllm_paged_attention(fdllm_handle* h, const fdllm_paged_cache* cache, int layer,
+                                    const fdllm_paged_plan* plan, const int32_t* plan_words, const int32_t* table,
+                                    int table_ld, const void* q, int ldq, float scale, void* out, void* stream);
+
+/* Log probabilities of given tokens, with entropy and top alternatives, from logits [rows, vocab]
+ * (logits_dtype FDLLM_FLOAT32 or FDLLM_BFLOAT16, row stride ld elements).  The reference reduces
+ * logits on the host (runners.py:877-881).  Per row, in fp32: lse = log sum exp(logits);
+ *   logprob[row] = logits[target] - lse          (targets int32; outside [0, vocab): device error 4, NaN)
+ *   entropy[row] = lse - sum softmax * logits    (nats; ids at -inf contribute nothing)
+ *   top_ids / top_logprobs [rows, top]           the `top` (0..32, <= vocab) largest logits in order,
+ *                                                ties to the lowest id, and their log probabilities.
+ * targets + logprob, entropy and top_* may be NULL.  A row with a NaN logit, a +inf logit or only
+ * -inf logits has NaN log probabilities and entropy; its ids order NaN as -inf. */
+FDLLM_API int fdllm_logprobs(fdllm_handle* h, const void* logits, int logits_dtype, int rows, int vocab, long long ld,
+                             const int32_t* targets, int top, float* logprob, float* entropy, int32_t* top_ids,
+                             float* top_logprobs, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
