@@ -210,6 +210,9 @@ struct fdllm_handle {
   DevBuf<float> attn_part, attn_part_lse;  // tcgen05 key-split partials
   DevBuf<float> persist_part;               // persistent-GEMM split-K partial tiles
   DevBuf<unsigned> persist_ctr;             // persistent-GEMM per-tile split counters (zero between launches)
+  DevBuf<float4> logprob_part;              // log-probability partials of a row's parts
+  DevBuf<unsigned long long> logprob_keys;  //   and their alternatives
+  DevBuf<unsigned> logprob_ctr;             //   and its arrived parts (zero between launches)
   // kernel trace (fdllm_kernel_trace_enable / _read): phase stamps of every projection and
   // attention launch issued outside stream capture while enabled, 8 per launch, and their kinds
   bool ktrace_on = false;

@@ -741,6 +741,9 @@ int fdllm_destroy(fdllm_handle* h) {
   for (auto* b : {&h->conf_part, &h->tmp_maxp, &h->ss, &h->dec.cmax}) b->release();
   h->persist_part.release();
   h->persist_ctr.release();
+  h->logprob_part.release();
+  h->logprob_keys.release();
+  h->logprob_ctr.release();
   h->ktrace.release();
   h->attn_maps.release();
   h->reqs.release();

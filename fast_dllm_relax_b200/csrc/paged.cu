@@ -232,10 +232,35 @@ int fdllm_logprobs(fdllm_handle* h, const void* logits, int logits_dtype, int ro
     if ((targets == nullptr) != (logprob == nullptr)) return fail(FDLLM_ERR_INVALID, "targets and logprob go together");
     if (top > 0 && (top_ids == nullptr || top_logprobs == nullptr)) return fail(FDLLM_ERR_INVALID, "null top outputs");
     if (logits == nullptr) return fail(FDLLM_ERR_INVALID, "null logits");
-    LogprobArgs a{logits, rows, vocab, ld, targets, top, logprob, entropy, top_ids, top_logprobs, nullptr};
+    LogprobArgs a{};
+    a.logits = logits;
+    a.rows = rows;
+    a.vocab = vocab;
+    a.ld = ld;
+    a.targets = targets;
+    a.top = top;
+    a.logprob = logprob;
+    a.entropy = entropy;
+    a.top_ids = top_ids;
+    a.top_logprobs = top_logprobs;
+    int part_chunks = 0;
+    const int parts = logprobs_parts(rows, vocab, logits_dtype, h->num_sms, &part_chunks);
+    if (static_cast<long long>(rows) * parts > 0x7FFFFFFFLL) return fail(FDLLM_ERR_INVALID, "too many logits");
     std::lock_guard<std::mutex> lock(h->mu);
+    if (parts > 1) {
+      const size_t n = static_cast<size_t>(rows) * parts;
+      FDLLM_TRY(h->logprob_part.ensure(n));
+      FDLLM_TRY(h->logprob_keys.ensure(n * std::max(top, 1)));
+      if (h->logprob_ctr.n < static_cast<size_t>(rows)) {  // zeroed in the order of this call's stream
+        FDLLM_TRY(h->logprob_ctr.ensure(rows));
+        CUDA_TRY(cudaMemsetAsync(h->logprob_ctr.p, 0, h->logprob_ctr.bytes(), static_cast<cudaStream_t>(stream)));
+      }
+      a.part = h->logprob_part.p;
+      a.keys = h->logprob_keys.p;
+      a.arrived = h->logprob_ctr.p;
+    }
     a.err = h->err.p;
-    CUDA_TRY(launch_logprobs(a, logits_dtype, static_cast<cudaStream_t>(stream)));
+    CUDA_TRY(launch_logprobs(a, logits_dtype, parts, part_chunks, static_cast<cudaStream_t>(stream)));
     return FDLLM_OK;
   });
 }

@@ -82,12 +82,17 @@ struct LogprobArgs {
   float *logprob, *entropy;
   int* top_ids;
   float* top_logprobs;
+  float4* part;               // [rows][parts] partial statistics
+  unsigned long long* keys;   // [rows][parts][top] partial alternatives
+  unsigned* arrived;          // [rows] parts done (zero between launches)
   int* err;
 };
 
 int launch_paged_append(const PagedAppendArgs& a, int dtype, cudaStream_t s);
 int launch_paged_attention_simt(const PagedAttnArgs& a, int dtype, cudaStream_t s);
-int launch_logprobs(const LogprobArgs& a, int dtype, cudaStream_t s);
+// CTAs a row is split into, and chunks each.
+int logprobs_parts(int rows, int vocab, int dtype, int num_sms, int* part_chunks);
+int launch_logprobs(const LogprobArgs& a, int dtype, int parts, int part_chunks, cudaStream_t s);
 
 #ifdef __CUDACC__
 // ---- float8 e4m3 (1 sign, 4 exponent, 3 mantissa bits; largest 448, no infinities) --------------
