@@ -210,6 +210,8 @@ struct fdllm_handle {
   DevBuf<float> attn_part, attn_part_lse;  // tcgen05 key-split partials
   DevBuf<float> persist_part;               // persistent-GEMM split-K partial tiles
   DevBuf<unsigned> persist_ctr;             // persistent-GEMM per-tile split counters (zero between launches)
+  DevBuf<float4> paged_part;                // paged attention: partials of tiles whose keys are split
+  DevBuf<unsigned> paged_ctr;               //   and their arrived items (zero between launches)
   DevBuf<float4> logprob_part;              // log-probability partials of a row's parts
   DevBuf<unsigned long long> logprob_keys;  //   and their alternatives
   DevBuf<unsigned> logprob_ctr;             //   and its arrived parts (zero between launches)

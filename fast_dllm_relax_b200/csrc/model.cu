@@ -741,6 +741,8 @@ int fdllm_destroy(fdllm_handle* h) {
   for (auto* b : {&h->conf_part, &h->tmp_maxp, &h->ss, &h->dec.cmax}) b->release();
   h->persist_part.release();
   h->persist_ctr.release();
+  h->paged_part.release();
+  h->paged_ctr.release();
   h->logprob_part.release();
   h->logprob_keys.release();
   h->logprob_ctr.release();

@@ -31,6 +31,15 @@ bool page_size_ok(int p) { return p == 16 || p == 32 || p == 64 || p == 128; }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
+// At least n arrival counters: zero when allocated (in the order of the call's stream), and again after
+// every launch that uses them.
+int ensure_counters(DevBuf<unsigned>* b, size_t n, cudaStream_t s) {
+  if (b->n >= n) return FDLLM_OK;
+  FDLLM_TRY(b->ensure(n));
+  CUDA_TRY(cudaMemsetAsync(b->p, 0, b->bytes(), s));
+  return FDLLM_OK;
+}
+
 // Rows of `cols` elements with a row stride of ld elements, every row 16-byte aligned.
 int check_rows(const fdllm_handle* h, const char* name, const void* p, int ld, int cols) {
   if (p == nullptr) return fail(FDLLM_ERR_INVALID, std::string(name) + ": null pointer");
@@ -61,6 +70,70 @@ int check_paged(const fdllm_handle* h, const fdllm_paged_cache* c, int layer, co
   const size_t heads = static_cast<size_t>(c->pages) * h->cfg.num_key_value_heads;
   *layer_scales = static_cast<size_t>(layer) * heads;
   *layer_codes = static_cast<size_t>(layer) * heads * c->page_size * h->cfg.head_dim;
+  return FDLLM_OK;
+}
+
+// Key shares of a tile that attends `keys` keys: of at least `share` keys, at most kMaxSplits of them.
+constexpr int kMaxSplits = 32;   // the last item of a tile reads them all
+constexpr int kMinShare = 256;
+constexpr int kShareUnit = 64;
+
+// The attention items of a bf16 batch.  Shares are sized so that the items fill the SMs a few times over.
+struct ItemPlan {
+  std::vector<PagedItem> items[kPagedClasses];
+  int tiles = 0;
+  long long parts = 0;
+};
+
+int plan_items(const fdllm_handle* h, const std::vector<PagedReq>& reqs, int causal_block, ItemPlan* out) {
+  const fdllm_config& c = h->cfg;
+  const int G = c.num_attention_heads / c.num_key_value_heads;
+  auto cls_of = [&](long long rows) { return rows <= 8 ? 0 : rows <= 16 ? 1 : 2; };
+  auto tile_rows = [](int cls) { return 8 * (cls + 1); };
+  auto keys_of = [&](const PagedReq& r, long long row_end) {  // keys of a tile whose last row is row_end - 1
+    const long long pos = r.start + (row_end - 1) / G;
+    return causal_block > 0 ? static_cast<int>(std::min<long long>(r.len, (pos / causal_block + 1) * causal_block)) : r.len;
+  };
+  long long work = 0;  // keys of all tiles and heads
+  for (const PagedReq& r : reqs) {
+    const long long rows = static_cast<long long>(r.rows) * G;
+    const int step = tile_rows(cls_of(rows));
+    for (long long t = 0; t < rows; t += step) work += static_cast<long long>(keys_of(r, std::min(rows, t + step))) * c.num_key_value_heads;
+  }
+  const long long target = 6LL * h->num_sms;
+  const long long share = std::max<long long>(kMinShare, (work / target + kShareUnit - 1) / kShareUnit * kShareUnit);
+  for (size_t i = 0; i < reqs.size(); ++i) {
+    const PagedReq& r = reqs[i];
+    const long long rows = static_cast<long long>(r.rows) * G;
+    const int cls = cls_of(rows), step = tile_rows(cls);
+    for (long long t = 0; t < rows; t += step) {
+      const int keys = keys_of(r, std::min(rows, t + step));
+      const int want = static_cast<int>(std::min<long long>(kMaxSplits, (keys + share - 1) / share));
+      const int each = ((keys + want - 1) / want + kShareUnit - 1) / kShareUnit * kShareUnit;
+      const int splits = (keys + each - 1) / each;
+      const int part = step * (c.head_dim / 4) + step;  // 16-byte units
+      for (int head = 0; head < c.num_key_value_heads; ++head) {
+        for (int s = 0; s < splits; ++s) {
+          PagedItem it{};
+          it.req = static_cast<int>(i);
+          it.row0 = static_cast<int>(t);
+          it.head = head;
+          it.key0 = s * each;
+          it.key1 = std::min(keys, (s + 1) * each);
+          it.split = s;
+          it.splits = splits;
+          it.tile = out->tiles;
+          it.part = splits > 1 ? static_cast<int>(out->parts + static_cast<long long>(s) * part) : 0;
+          out->items[cls].push_back(it);
+        }
+        if (splits > 1) {
+          out->parts += static_cast<long long>(splits) * part;
+          ++out->tiles;
+        }
+        if (out->parts > 0x7FFFFFFFLL) return fail(FDLLM_ERR_INVALID, "batch too large for one plan");
+      }
+    }
+  }
   return FDLLM_OK;
 }
 
@@ -106,6 +179,15 @@ int fdllm_paged_plan_batch(fdllm_handle* h, const int32_t* rows, const int32_t* 
     out.priv[kPagedPageUnits] = static_cast<int>(units.size());
     out.priv[kPagedPageOff] = at;
     at += 2 * static_cast<int>(units.size());
+    ItemPlan ip;
+    if (h->dtype == FDLLM_BFLOAT16) FDLLM_TRY(plan_items(h, reqs, causal_block, &ip));
+    out.priv[kPagedTiles] = ip.tiles;
+    out.priv[kPagedParts] = static_cast<int>(ip.parts);
+    for (int c = 0; c < kPagedClasses; ++c) {
+      out.priv[kPagedItems + c] = static_cast<int>(ip.items[c].size());
+      out.priv[kPagedItemOff + c] = at;
+      at += kPagedItemWords * static_cast<int>(ip.items[c].size());
+    }
     out.words = at;
     *plan = out;
     if (cap < at) {
@@ -115,6 +197,9 @@ int fdllm_paged_plan_batch(fdllm_handle* h, const int32_t* rows, const int32_t* 
     if (n > 0) std::memcpy(words, reqs.data(), reqs.size() * sizeof(PagedReq));
     if (!units.empty())
       std::memcpy(words + out.priv[kPagedPageOff], units.data(), units.size() * sizeof(PagedPageUnit));
+    for (int c = 0; c < kPagedClasses; ++c)
+      if (!ip.items[c].empty())
+        std::memcpy(words + out.priv[kPagedItemOff + c], ip.items[c].data(), ip.items[c].size() * sizeof(PagedItem));
     return FDLLM_OK;
   });
 }
@@ -202,6 +287,7 @@ int fdllm_paged_attention(fdllm_handle* h, const fdllm_paged_cache* cache, int l
     a.v_scale = cache->v_scale + scales;
     a.pages = cache->pages;
     a.page_size = cache->page_size;
+    while ((1 << a.page_shift) < a.page_size) ++a.page_shift;
     a.hq = c.num_attention_heads;
     a.hkv = c.num_key_value_heads;
     a.hd = c.head_dim;
@@ -212,7 +298,20 @@ int fdllm_paged_attention(fdllm_handle* h, const fdllm_paged_cache* cache, int l
     a.out = out;
     std::lock_guard<std::mutex> lock(h->mu);
     a.err = h->err.p;
-    CUDA_TRY(launch_paged_attention_simt(a, h->dtype, static_cast<cudaStream_t>(stream)));
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (h->dtype != FDLLM_BFLOAT16) {
+      CUDA_TRY(launch_paged_attention_simt(a, st));
+      return FDLLM_OK;
+    }
+    FDLLM_TRY(h->paged_part.ensure(plan->priv[kPagedParts]));
+    FDLLM_TRY(ensure_counters(&h->paged_ctr, plan->priv[kPagedTiles], st));
+    a.part = h->paged_part.p;
+    a.arrived = h->paged_ctr.p;
+    for (int c = 0; c < kPagedClasses; ++c) {
+      if (plan->priv[kPagedItems + c] == 0) continue;
+      a.items = reinterpret_cast<const PagedItem*>(plan_words + plan->priv[kPagedItemOff + c]);
+      CUDA_TRY(launch_paged_attention_narrow(a, c + 1, plan->priv[kPagedItems + c], st));
+    }
     return FDLLM_OK;
   });
 }
@@ -251,10 +350,7 @@ int fdllm_logprobs(fdllm_handle* h, const void* logits, int logits_dtype, int ro
       const size_t n = static_cast<size_t>(rows) * parts;
       FDLLM_TRY(h->logprob_part.ensure(n));
       FDLLM_TRY(h->logprob_keys.ensure(n * std::max(top, 1)));
-      if (h->logprob_ctr.n < static_cast<size_t>(rows)) {  // zeroed in the order of this call's stream
-        FDLLM_TRY(h->logprob_ctr.ensure(rows));
-        CUDA_TRY(cudaMemsetAsync(h->logprob_ctr.p, 0, h->logprob_ctr.bytes(), static_cast<cudaStream_t>(stream)));
-      }
+      FDLLM_TRY(ensure_counters(&h->logprob_ctr, rows, static_cast<cudaStream_t>(stream)));
       a.part = h->logprob_part.p;
       a.keys = h->logprob_keys.p;
       a.arrived = h->logprob_ctr.p;

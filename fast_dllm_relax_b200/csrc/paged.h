@@ -29,10 +29,30 @@ struct PagedPageUnit {
   int slot;  // page number within the request
 };
 
+// One share of an attention call (bf16): query rows [row0, ..) of a request and KV head (row = token * G +
+// query head within the group) over keys [key0, key1).  The items of one tile (same rows) are consecutive.
+constexpr int kPagedItemWords = 10;
+struct PagedItem {
+  int req, row0, head;  // head: KV head
+  int key0, key1;       // key0 a multiple of 64
+  int split, splits;    // this share's number and how many the tile has
+  int tile;             // arrival counter
+  int part;             // its partial in the workspace, in 16-byte units (splits > 1)
+  int pad;
+};
+static_assert(sizeof(PagedItem) == 4 * kPagedItemWords, "plan item layout");
+
+// Item classes, a launch each: tiles of 8, 16 and 24 query rows.
+constexpr int kPagedClasses = 3;
+
 // fdllm_paged_plan::priv
 enum PagedPriv : int {
   kPagedPageUnits = 0,  // number of page units
   kPagedPageOff = 1,    // word offset of the page units
+  kPagedTiles = 2,      // arrival counters needed
+  kPagedParts = 3,      // workspace for partials, in 16-byte units
+  kPagedItems = 4,      // [kPagedClasses] numbers of items
+  kPagedItemOff = kPagedItems + kPagedClasses,  // [kPagedClasses] word offsets of the items
 };
 
 struct PagedAppendArgs {
@@ -61,13 +81,16 @@ struct PagedAttnArgs {
   int table_ld;
   const uint8_t *k, *v;
   const float *k_scale, *v_scale;
-  int pages, page_size;
+  int pages, page_size, page_shift;  // page_size = 1 << page_shift
   int hq, hkv, hd;
   int causal_block;
   const void* q;
   int ldq;
   float scale;
   void* out;
+  const PagedItem* items;
+  float4* part;        // partials of split tiles
+  unsigned* arrived;   // [tiles] items done (zero between launches)
   int* err;
 };
 
@@ -89,7 +112,8 @@ struct LogprobArgs {
 };
 
 int launch_paged_append(const PagedAppendArgs& a, int dtype, cudaStream_t s);
-int launch_paged_attention_simt(const PagedAttnArgs& a, int dtype, cudaStream_t s);
+int launch_paged_attention_simt(const PagedAttnArgs& a, cudaStream_t s);  // fp32
+int launch_paged_attention_narrow(const PagedAttnArgs& a, int nt, int n_items, cudaStream_t s);
 // CTAs a row is split into, and chunks each.
 int logprobs_parts(int rows, int vocab, int dtype, int num_sms, int* part_chunks);
 int launch_logprobs(const LogprobArgs& a, int dtype, int parts, int part_chunks, cudaStream_t s);

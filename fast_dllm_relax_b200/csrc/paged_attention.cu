@@ -1,5 +1,4 @@
-// Attention over a paged 8-bit KV cache (fdllm_paged_attention) on CUDA cores: any dtype and head
-// layout.  Reference semantics: runtime.py:63-73 (every query row attends the cached rows), with the
+// Attention over a paged 8-bit KV cache (fdllm_paged_attention) on CUDA cores, for fp32 queries.  Reference semantics: runtime.py:63-73 (every query row attends the cached rows), with the
 // cache's values code * scale.
 //
 // One CTA of four warps per (token row, query head).  Each warp walks its share of the keys with the
@@ -78,8 +77,6 @@ int launch_simt(const PagedAttnArgs& a, cudaStream_t s) {
 
 }  // namespace
 
-int launch_paged_attention_simt(const PagedAttnArgs& a, int dtype, cudaStream_t s) {
-  return dtype == 1 ? launch_simt<bf16>(a, s) : launch_simt<float>(a, s);
-}
+int launch_paged_attention_simt(const PagedAttnArgs& a, cudaStream_t s) { return launch_simt<float>(a, s); }
 
 }  // namespace fdllm
