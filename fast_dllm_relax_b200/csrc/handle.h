@@ -247,6 +247,9 @@ void release_step_graphs(fdllm_handle* h);
 int dense_forward(fdllm_handle* h, const void* x, const float* bias, int T, void* k, void* v, int cap, bool scratch,
                   void* out, cudaStream_t s);
 int cached_desc(fdllm_handle* h, const fdllm_request& r, int q_tok0, ReqDesc* d);
+// 2D uint8 map of a paged cache's codes as rows of head_dim bytes, box one page (at most 64 rows), 128-byte
+// swizzle at head_dim 128.
+int make_page_map(CUtensorMap* map, const void* base, const fdllm_paged_cache* c, int kv_heads, int head_dim);
 int confidence_locked(fdllm_handle* h, const void* hidden, int rows, int32_t* ids, float* maxp,
                       const int32_t* targets, float* logprob, cudaStream_t s);
 

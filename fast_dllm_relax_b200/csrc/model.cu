@@ -101,6 +101,22 @@ static int make_kv_map(CUtensorMap* map, const void* base, int cols, int keys, i
   return FDLLM_OK;
 }
 
+int fdllm::make_page_map(CUtensorMap* map, const void* base, const fdllm_paged_cache* c, int kv_heads, int head_dim) {
+  EncodeTiledFn fn = encode_fn();
+  if (fn == nullptr) return fail(FDLLM_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+  const unsigned long long rows = static_cast<unsigned long long>(c->layers) * c->pages * kv_heads * c->page_size;
+  if (rows > 0x7FFFFFFFull) return fail(FDLLM_ERR_UNSUPPORTED, "paged cache exceeds 2^31 rows");  // TMA coordinates are int32
+  cuuint64_t dims[2] = {static_cast<cuuint64_t>(head_dim), rows};
+  cuuint64_t strides[1] = {static_cast<cuuint64_t>(head_dim)};
+  cuuint32_t box[2] = {static_cast<cuuint32_t>(head_dim), static_cast<cuuint32_t>(std::min(c->page_size, 64))};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, head_dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(FDLLM_ERR_CUDA, "cuTensorMapEncodeTiled (pages) failed (" + std::to_string(r) + ")");
+  return FDLLM_OK;
+}
+
 size_t fdllm::round_up(size_t x, size_t m) { return (x + m - 1) / m * m; }
 
 // "key=value,key=value" over the Tuning fields; unknown keys or values out of range fail.

@@ -64,6 +64,7 @@ int check_paged(const fdllm_handle* h, const fdllm_paged_cache* c, int layer, co
     return fail(FDLLM_ERR_INVALID, "the plan is for pages of " + std::to_string(p->page_size) + " rows, the cache has " +
                                        std::to_string(c->page_size));
   if (p->total_rows > 0 && (words == nullptr || table == nullptr)) return fail(FDLLM_ERR_INVALID, "null plan words or table");
+  if (!aligned16(words)) return fail(FDLLM_ERR_INVALID, "plan words must be 16-byte aligned");
   if (table_ld < p->table_cols)
     return fail(FDLLM_ERR_INVALID, "page table has " + std::to_string(table_ld) + " columns; the longest request needs " +
                                        std::to_string(p->table_cols));
@@ -73,51 +74,74 @@ int check_paged(const fdllm_handle* h, const fdllm_paged_cache* c, int layer, co
   return FDLLM_OK;
 }
 
-// Key shares of a tile that attends `keys` keys: of at least `share` keys, at most kMaxSplits of them.
-constexpr int kMaxSplits = 32;   // the last item of a tile reads them all
-constexpr int kMinShare = 256;
-constexpr int kShareUnit = 64;
+constexpr int kMaxSplits = 32;   // key shares of a tile: its last item reads them all
+constexpr int kMinShare = 256;   // keys
+constexpr int kShareUnit = 128;
 
-// The attention items of a bf16 batch.  Shares are sized so that the items fill the SMs a few times over.
+// The attention items of a bf16 batch.
 struct ItemPlan {
   std::vector<PagedItem> items[kPagedClasses];
   int tiles = 0;
   long long parts = 0;
 };
 
+// Rows of a request and KV head are cut into equal tiles of a class's size.  Keys are cut into shares only
+// as far as that fills the SMs (`slots` CTAs are resident at once): a share costs its prologue, its partial
+// and a part of the join, so shares grow until the items fit one wave.
 int plan_items(const fdllm_handle* h, const std::vector<PagedReq>& reqs, int causal_block, ItemPlan* out) {
   const fdllm_config& c = h->cfg;
-  const int G = c.num_attention_heads / c.num_key_value_heads;
-  auto cls_of = [&](long long rows) { return rows <= 8 ? 0 : rows <= 16 ? 1 : 2; };
-  auto tile_rows = [](int cls) { return 8 * (cls + 1); };
+  const int G = c.num_attention_heads / c.num_key_value_heads, heads = c.num_key_value_heads;
+  const bool tc = c.head_dim == 128;
+  const int unit = tc ? 16 : 8, largest = tc ? 48 : 24;
+  const long long slots = (tc ? 2LL : 3LL) * h->num_sms;
+  auto tile_rows = [&](long long rows) {
+    const long long tiles = (rows + largest - 1) / largest;
+    return static_cast<int>(((rows + tiles - 1) / tiles + unit - 1) / unit * unit);
+  };
   auto keys_of = [&](const PagedReq& r, long long row_end) {  // keys of a tile whose last row is row_end - 1
     const long long pos = r.start + (row_end - 1) / G;
     return causal_block > 0 ? static_cast<int>(std::min<long long>(r.len, (pos / causal_block + 1) * causal_block)) : r.len;
   };
-  long long work = 0;  // keys of all tiles and heads
+  auto splits_of = [&](int keys, long long share) { return static_cast<int>(std::min<long long>(kMaxSplits, (keys + share - 1) / share)); };
+  std::vector<int> tile_keys;  // of every tile of one head
+  long long work = 0, longest = 0;
   for (const PagedReq& r : reqs) {
     const long long rows = static_cast<long long>(r.rows) * G;
-    const int step = tile_rows(cls_of(rows));
-    for (long long t = 0; t < rows; t += step) work += static_cast<long long>(keys_of(r, std::min(rows, t + step))) * c.num_key_value_heads;
+    const int step = rows > 0 ? tile_rows(rows) : 1;
+    for (long long t = 0; t < rows; t += step) {
+      tile_keys.push_back(keys_of(r, std::min(rows, t + step)));
+      work += tile_keys.back();
+      longest = std::max<long long>(longest, tile_keys.back());
+    }
   }
-  const long long target = 6LL * h->num_sms;
-  const long long share = std::max<long long>(kMinShare, (work / target + kShareUnit - 1) / kShareUnit * kShareUnit);
+  long long share = std::max<long long>(kMinShare, (work * heads / slots + kShareUnit) / kShareUnit * kShareUnit);
+  while (share < longest) {
+    long long items = 0;
+    for (int k : tile_keys) items += splits_of(k, share);
+    if (items * heads <= slots) break;
+    share += (share / 16 + kShareUnit) / kShareUnit * kShareUnit;
+  }
   for (size_t i = 0; i < reqs.size(); ++i) {
     const PagedReq& r = reqs[i];
     const long long rows = static_cast<long long>(r.rows) * G;
-    const int cls = cls_of(rows), step = tile_rows(cls);
+    if (rows == 0) continue;
+    const int step = tile_rows(rows), cls = step / unit - 1;
     for (long long t = 0; t < rows; t += step) {
       const int keys = keys_of(r, std::min(rows, t + step));
-      const int want = static_cast<int>(std::min<long long>(kMaxSplits, (keys + share - 1) / share));
+      const int want = splits_of(keys, share);
       const int each = ((keys + want - 1) / want + kShareUnit - 1) / kShareUnit * kShareUnit;
       const int splits = (keys + each - 1) / each;
       const int part = step * (c.head_dim / 4) + step;  // 16-byte units
-      for (int head = 0; head < c.num_key_value_heads; ++head) {
+      for (int head = 0; head < heads; ++head) {
         for (int s = 0; s < splits; ++s) {
           PagedItem it{};
           it.req = static_cast<int>(i);
-          it.row0 = static_cast<int>(t);
           it.head = head;
+          it.row0 = static_cast<int>(t);
+          it.rows = static_cast<int>(std::min<long long>(step, rows - t));
+          it.tok0 = r.tok0;
+          it.start = r.start;
+          it.len = r.len;
           it.key0 = s * each;
           it.key1 = std::min(keys, (s + 1) * each);
           it.split = s;
@@ -134,6 +158,9 @@ int plan_items(const fdllm_handle* h, const std::vector<PagedReq>& reqs, int cau
       }
     }
   }
+  // longest items first: the last CTAs to start are the short ones
+  for (auto& v : out->items)
+    std::stable_sort(v.begin(), v.end(), [](const PagedItem& a, const PagedItem& b) { return a.key1 - a.key0 > b.key1 - b.key0; });
   return FDLLM_OK;
 }
 
@@ -179,6 +206,7 @@ int fdllm_paged_plan_batch(fdllm_handle* h, const int32_t* rows, const int32_t* 
     out.priv[kPagedPageUnits] = static_cast<int>(units.size());
     out.priv[kPagedPageOff] = at;
     at += 2 * static_cast<int>(units.size());
+    at = (at + 3) & ~3;  // items are read in 16-byte words
     ItemPlan ip;
     if (h->dtype == FDLLM_BFLOAT16) FDLLM_TRY(plan_items(h, reqs, causal_block, &ip));
     out.priv[kPagedTiles] = ip.tiles;
@@ -194,6 +222,7 @@ int fdllm_paged_plan_batch(fdllm_handle* h, const int32_t* rows, const int32_t* 
       if (cap == 0 && words == nullptr) return FDLLM_OK;  // size query
       return fail(FDLLM_ERR_INVALID, "plan needs " + std::to_string(at) + " words, given " + std::to_string(cap));
     }
+    std::memset(words, 0, sizeof(int32_t) * at);
     if (n > 0) std::memcpy(words, reqs.data(), reqs.size() * sizeof(PagedReq));
     if (!units.empty())
       std::memcpy(words + out.priv[kPagedPageOff], units.data(), units.size() * sizeof(PagedPageUnit));
@@ -305,12 +334,18 @@ int fdllm_paged_attention(fdllm_handle* h, const fdllm_paged_cache* cache, int l
     }
     FDLLM_TRY(h->paged_part.ensure(plan->priv[kPagedParts]));
     FDLLM_TRY(ensure_counters(&h->paged_ctr, plan->priv[kPagedTiles], st));
+    CUtensorMap tm_k, tm_v;
+    FDLLM_TRY(make_page_map(&tm_k, cache->k, cache, c.num_key_value_heads, c.head_dim));
+    FDLLM_TRY(make_page_map(&tm_v, cache->v, cache, c.num_key_value_heads, c.head_dim));
+    a.layer_row = static_cast<int>(codes / c.head_dim);
     a.part = h->paged_part.p;
     a.arrived = h->paged_ctr.p;
-    for (int c = 0; c < kPagedClasses; ++c) {
-      if (plan->priv[kPagedItems + c] == 0) continue;
-      a.items = reinterpret_cast<const PagedItem*>(plan_words + plan->priv[kPagedItemOff + c]);
-      CUDA_TRY(launch_paged_attention_narrow(a, c + 1, plan->priv[kPagedItems + c], st));
+    for (int k = 0; k < kPagedClasses; ++k) {
+      if (plan->priv[kPagedItems + k] == 0) continue;
+      a.items = reinterpret_cast<const PagedItem*>(plan_words + plan->priv[kPagedItemOff + k]);
+      const int n = plan->priv[kPagedItems + k];
+      CUDA_TRY(c.head_dim == 128 ? launch_paged_attention_tc(a, 16 * (k + 1), n, tm_k, tm_v, st)
+                                 : launch_paged_attention_narrow(a, k + 1, n, tm_k, tm_v, st));
     }
     return FDLLM_OK;
   });

@@ -31,18 +31,21 @@ struct PagedPageUnit {
 
 // One share of an attention call (bf16): query rows [row0, ..) of a request and KV head (row = token * G +
 // query head within the group) over keys [key0, key1).  The items of one tile (same rows) are consecutive.
-constexpr int kPagedItemWords = 10;
-struct PagedItem {
-  int req, row0, head;  // head: KV head
-  int key0, key1;       // key0 a multiple of 64
+constexpr int kPagedItemWords = 16;
+struct alignas(16) PagedItem {
+  int req, head;        // head: KV head
+  int row0, rows;       // rows [row0, row0 + rows) of the request and KV head
+  int key0, key1;       // key0 a multiple of 128
+  int tok0, start, len; // the request's (PagedReq)
   int split, splits;    // this share's number and how many the tile has
   int tile;             // arrival counter
   int part;             // its partial in the workspace, in 16-byte units (splits > 1)
-  int pad;
+  int pad[3];
 };
 static_assert(sizeof(PagedItem) == 4 * kPagedItemWords, "plan item layout");
 
-// Item classes, a launch each: tiles of 8, 16 and 24 query rows.
+// Item classes, a launch each: tiles of 16, 32 and 48 query rows at head_dim 128 (tcgen05), of 8, 16 and 24 at
+// the others (mma.sync).
 constexpr int kPagedClasses = 3;
 
 // fdllm_paged_plan::priv
@@ -89,6 +92,7 @@ struct PagedAttnArgs {
   float scale;
   void* out;
   const PagedItem* items;
+  int layer_row;       // first row of this layer in the pool's maps (rows of head_dim codes)
   float4* part;        // partials of split tiles
   unsigned* arrived;   // [tiles] items done (zero between launches)
   int* err;
@@ -113,7 +117,10 @@ struct LogprobArgs {
 
 int launch_paged_append(const PagedAppendArgs& a, int dtype, cudaStream_t s);
 int launch_paged_attention_simt(const PagedAttnArgs& a, cudaStream_t s);  // fp32
-int launch_paged_attention_narrow(const PagedAttnArgs& a, int nt, int n_items, cudaStream_t s);
+int launch_paged_attention_narrow(const PagedAttnArgs& a, int nt, int n_items, const CUtensorMap& k, const CUtensorMap& v,
+                                  cudaStream_t s);
+int launch_paged_attention_tc(const PagedAttnArgs& a, int cols, int n_items, const CUtensorMap& k, const CUtensorMap& v,
+                              cudaStream_t s);
 // CTAs a row is split into, and chunks each.
 int logprobs_parts(int rows, int vocab, int dtype, int num_sms, int* part_chunks);
 int launch_logprobs(const LogprobArgs& a, int dtype, int parts, int part_chunks, cudaStream_t s);
