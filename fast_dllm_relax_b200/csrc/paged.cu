@@ -74,7 +74,6 @@ int check_paged(const fdllm_handle* h, const fdllm_paged_cache* c, int layer, co
   return FDLLM_OK;
 }
 
-constexpr int kMaxSplits = 32;   // key shares of a tile: its last item reads them all
 constexpr int kMinShare = 256;   // keys
 constexpr int kShareUnit = 128;
 
@@ -102,7 +101,7 @@ int plan_items(const fdllm_handle* h, const std::vector<PagedReq>& reqs, int cau
     const long long pos = r.start + (row_end - 1) / G;
     return causal_block > 0 ? static_cast<int>(std::min<long long>(r.len, (pos / causal_block + 1) * causal_block)) : r.len;
   };
-  auto splits_of = [&](int keys, long long share) { return static_cast<int>(std::min<long long>(kMaxSplits, (keys + share - 1) / share)); };
+  auto splits_of = [&](int keys, long long share) { return static_cast<int>(std::min<long long>(kMaxPagedSplits, (keys + share - 1) / share)); };
   std::vector<int> tile_keys;  // of every tile of one head
   long long work = 0, longest = 0;
   for (const PagedReq& r : reqs) {

@@ -29,6 +29,8 @@ struct PagedPageUnit {
   int slot;  // page number within the request
 };
 
+constexpr int kMaxPagedSplits = 32;  // key shares of a tile (a lane each in the join)
+
 // One share of an attention call (bf16): query rows [row0, ..) of a request and KV head (row = token * G +
 // query head within the group) over keys [key0, key1).  The items of one tile (same rows) are consecutive.
 constexpr int kPagedItemWords = 16;

@@ -13,16 +13,16 @@
 // power of two per row (largest element in [2^7, 2^8)), exact for elements above 2^-10 of the row's largest and
 // to 2^-18 of it below; two 8-bit products cost one 16-bit product's time, and K needs no widening.  P would
 // need three e4m3 terms to keep small weights, so the second product is in f16 (11 bits, weights down to 2^-32
-// of the largest), and a softmax thread widens its key's V row on the way (exact).  Each column's base B moves
-// only when a weight passes 2^kTrip (then its maximum sits at 2^kSeat): one block-wide vote a tile instead of a
-// maximum over 128 lanes.  log2 vs in the exponent keeps P in range whatever the page scales are; the row sums
-// take it back out.
+// of the largest), and V is widened on the way (exact).  Each column's base B moves only when a weight passes
+// 2^kTrip (then its maximum sits at 2^kSeat): one block-wide vote a tile instead of a maximum over 128 lanes.
+// log2 vs in the exponent keeps P in range whatever the page scales are; the row sums take it back out.
 //
-// Roles (192 threads): warp 0 the TMA producer (a lane a page; page ids and scales 32 pages at a time), warp 1
-// the MMA issuer and TMEM owner, warps 2-5 the softmax, a key a thread.  S^T is double-buffered, so S_{j+1} is
-// computed while tile j is in the softmax.  K and V have rings of their own: a V stage is free once widened,
-// a K stage once its scores are computed (up to 32 rows) or, where P replaces K in it to leave room for two
-// CTAs on an SM, once P is used.
+// Roles (384 threads, registers moved to the softmax): warp 0 the TMA producer (a lane a page; page ids and
+// scales 32 pages at a time), warp 1 the MMA issuer and TMEM owner, warps 4-7 the softmax, a key a thread, warps
+// 8-11 widen V, 64 keys at a time so that a half tile's product overlaps the other half's widening.  S^T is
+// double-buffered: S_{j+1} is computed while tile j is in the softmax.  K and V have rings of their own: a V
+// stage is free once widened, a K stage once its scores are computed (16 rows) or, where P replaces K in it to
+// leave room for two CTAs on an SM, once P is used.
 //
 // A tile whose keys are split over several items joins them through the workspace as in
 // paged_attention_narrow.cu: the last item to arrive adds the partials in item order.
@@ -125,16 +125,22 @@ struct Cfg {
   static_assert(kP <= kTile, "P replaces K in its stage");
 };
 
+constexpr int kThreads = 384;
+constexpr int kRegsLaunch = 80, kRegsMisc = 48, kRegsSoftmax = 144, kRegsWiden = 48;
+static_assert(kRegsMisc + kRegsSoftmax + kRegsWiden == 3 * kRegsLaunch, "the split is the launch's registers");
+
 template <int N>
 struct Bars {
   uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
-  uint64_t q_ready, s_full[2], s_free[2], p_full, pv_done, o_final;
+  uint64_t q_ready, s_full[2], s_free[2], p_full, w_full[2], pv_done[2], o_final;
   uint32_t tmem;
   int last;
   float2 scale[kStages][kKeys / 16];  // (K, V) scales of a stage's pages
-  alignas(16) float unscale[N], base[N], delta[N], factor[N];
+  alignas(16) float2 map[4][N];       // x = S a + c for a softmax warp's first page: (a, c) a column
+  float unscale[N], base[N], delta[N], factor[N];
   float part[4][N];  // a warp's column maxima, at the end its column sums
   int lim[N];
+  int out[N];        // (token, head) row of the output
 };
 template <int N>
 constexpr bool two_ctas() { return Cfg<N>::kBytes + static_cast<int>(sizeof(Bars<N>)) + 1024 <= 228 * 1024 / 2; }
@@ -142,8 +148,14 @@ static_assert(two_ctas<16>() && two_ctas<32>() && two_ctas<48>(), "two CTAs per 
 
 }  // namespace
 
+template <int kRegs, bool kGrow>
+__device__ __forceinline__ void set_registers() {
+  if constexpr (kGrow) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs));
+  else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs));
+}
+
 template <int N>
-__global__ void __launch_bounds__(192, 2)
+__global__ void __launch_bounds__(kThreads, 2)
     paged_attn_tc_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap tm_k,
                          const __grid_constant__ CUtensorMap tm_v) {
   using C = Cfg<N>;
@@ -158,15 +170,16 @@ __global__ void __launch_bounds__(192, 2)
       mbar_init(&b.k_full[i], 32);
       mbar_init(&b.k_empty[i], 1);
       mbar_init(&b.v_full[i], 32);
-      mbar_init(&b.v_empty[i], 4);
+      mbar_init(&b.v_empty[i], 8);
     }
-    mbar_init(&b.q_ready, 4);
+    mbar_init(&b.q_ready, 8);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&b.s_full[i], 1);
       mbar_init(&b.s_free[i], 4);
+      mbar_init(&b.w_full[i], 4);
+      mbar_init(&b.pv_done[i], 1);
     }
     mbar_init(&b.p_full, 4);
-    mbar_init(&b.pv_done, 1);
     mbar_init(&b.o_final, 1);
     mbar_fence_init();
   }
@@ -184,6 +197,57 @@ __global__ void __launch_bounds__(192, 2)
   const int G = a.hq / a.hkv;
   const int n_tiles = (it.key1 - it.key0 + kKeys - 1) / kKeys;
 
+  if (warp >= 4) {
+    // queries, by the softmax and widening warps: a warp a row, four head columns a lane, all loads in flight
+    constexpr int kQr = N / 8;
+    const int w8 = warp - 4;
+    uint2 raw[kQr];
+#pragma unroll
+    for (int i = 0; i < kQr; ++i) {
+      const int n = w8 + 8 * i, row = it.row0 + n;
+      raw[i] = make_uint2(0u, 0u);
+      if (n < it.rows)
+        raw[i] = *reinterpret_cast<const uint2*>(static_cast<const bf16*>(a.q) + static_cast<size_t>(it.tok0 + row / G) * a.ldq +
+                                                 static_cast<size_t>(it.head * G + row % G) * kHd + 4 * lane);
+    }
+#pragma unroll
+    for (int i = 0; i < kQr; ++i) {
+      const int n = w8 + 8 * i;
+      const uint2 u = raw[i];
+      const float x[4] = {__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xFFFF0000u), __uint_as_float(u.y << 16),
+                          __uint_as_float(u.y & 0xFFFF0000u)};
+      float m = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+      m = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m)));
+      // exponent of m, kept where both the scale and its inverse are normal floats
+      const int e = min(max(static_cast<int>(__float_as_uint(m) >> 23) - 127, -110), 110);
+      const float up = m > 0.f ? __uint_as_float(static_cast<uint32_t>(127 + 7 - e) << 23) : 1.f;
+      uint32_t hi = 0, lo = 0;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float x0 = x[2 * h] * up, x1 = x[2 * h + 1] * up;
+        const uint16_t c = e4m3x2_from_f32(x0, x1);
+        const float2 r = f32x2_from_e4m3x2(c);
+        hi |= static_cast<uint32_t>(c) << (16 * h);
+        lo |= static_cast<uint32_t>(e4m3x2_from_f32(x0 - r.x, x1 - r.y)) << (16 * h);
+      }
+      const int at = n * kHd + (((lane >> 2) ^ (n & 7)) << 4) + (lane & 3) * 4;  // 128-byte swizzle
+      *reinterpret_cast<uint32_t*>(sq + at) = hi;
+      *reinterpret_cast<uint32_t*>(sq + C::kQ + at) = lo;
+      if (lane == 0) {
+        const int row = it.row0 + n;
+        b.unscale[n] = a.scale * kLog2e / up;
+        b.base[n] = 0.f;
+        b.lim[n] = n < it.rows ? min(it.key1, paged_key_limit(it.len, it.start + row / G, a.causal_block)) : it.key1;
+        b.out[n] = (it.tok0 + row / G) * a.hq + it.head * G + row % G;
+      }
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&b.q_ready);
+    named_sync(3, 256);
+  }
+
+  if (warp < 4) set_registers<kRegsMisc, false>();
   if (warp == 0) {
     // ---------------- TMA producer: a lane a page ----------------
     const int ps = a.page_size, per_tile = kKeys >> a.page_shift, box = min(ps, 64);
@@ -267,62 +331,80 @@ __global__ void __launch_bounds__(192, 2)
             site = 45;
             break;
           }
-          tc_fence_after_sync();
           const uint8_t* p = C::kOwnP ? smem + C::kOffP + (i & 1) * C::kP : smem + C::kOffK + (i % kStages) * kTile;
 #pragma unroll
-          for (int k = 0; k < 8; ++k)  // 16 keys a step: two 8-row groups of V and of P
-            tc_mma_bf16(tmem + C::kO, umma_desc_sw128_mn(sv16 + k * 2048, kTile, 1024),
-                        umma_desc_mn(p + k * 256, kKeys * 16, 128), id_o, (i > 0 || k > 0) ? 1u : 0u);
-          tc_commit(&b.pv_done);
+          for (int h = 0; h < 2; ++h) {
+            if (!mbar_wait(&b.w_full[h], i & 1u)) {
+              site = 48;
+              break;
+            }
+            tc_fence_after_sync();
+#pragma unroll
+            for (int k = 4 * h; k < 4 * h + 4; ++k)  // 16 keys a step: two 8-row groups of V and of P
+              tc_mma_bf16(tmem + C::kO, umma_desc_sw128_mn(sv16 + k * 2048, kTile, 1024),
+                          umma_desc_mn(p + k * 256, kKeys * 16, 128), id_o, (i > 0 || k > 0) ? 1u : 0u);
+            tc_commit(&b.pv_done[h]);
+          }
+          if (site != 0) break;
           if (!C::kOwnP) tc_commit(&b.k_empty[i % kStages]);
           if (i == n_tiles - 1) tc_commit(&b.o_final);
         }
       }
       if (site != 0) report_wait(a.err, kErrTimeoutMma, site, a.total_rows, it.splits);
     }
-  } else {
-    // ---------------- softmax warps 2-5: a key a thread ----------------
-    const int q4 = warp & 3, tid = q4 * 32 + lane;  // TMEM lane
-    const uint32_t lane_base = static_cast<uint32_t>(q4 * 32) << 16;
-    // queries: a warp a row, four head columns a lane
-    for (int n = q4; n < N; n += 4) {
-      const int row = it.row0 + n;
-      const bool ok = n < it.rows;
-      float x[4] = {0.f, 0.f, 0.f, 0.f}, m = 0.f;
-      if (ok) {
-        const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const bf16*>(a.q) +
-                                                        static_cast<size_t>(it.tok0 + row / G) * a.ldq +
-                                                        static_cast<size_t>(it.head * G + row % G) * kHd + 4 * lane);
-        x[0] = __uint_as_float(u.x << 16), x[1] = __uint_as_float(u.x & 0xFFFF0000u);
-        x[2] = __uint_as_float(u.y << 16), x[3] = __uint_as_float(u.y & 0xFFFF0000u);
-        m = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
-      }
-      m = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m)));
-      // exponent of m, kept where both the scale and its inverse are normal floats
-      const int e = min(max(static_cast<int>(__float_as_uint(m) >> 23) - 127, -110), 110);
-      const float up = m > 0.f ? __uint_as_float(static_cast<uint32_t>(127 + 7 - e) << 23) : 1.f;
-      uint32_t hi = 0, lo = 0;
+  } else if (warp >= 8) {
+    set_registers<kRegsWiden, false>();
+    // ---------------- V in f16: a key a lane, half a row a thread, 64 keys at a time ----------------
+    const int half = warp & 1;
+    bool ok = true;
+    for (int j = 0; j < n_tiles && ok; ++j) {
+      const int st = j % kStages;
+      ok = __all_sync(0xffffffffu, mbar_wait(&b.v_full[st], (j / kStages) & 1u));
+      if (!ok) break;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const float x0 = x[2 * h] * up, x1 = x[2 * h + 1] * up;
-        const uint16_t c = e4m3x2_from_f32(x0, x1);
-        const float2 r = f32x2_from_e4m3x2(c);
-        hi |= static_cast<uint32_t>(c) << (16 * h);
-        lo |= static_cast<uint32_t>(e4m3x2_from_f32(x0 - r.x, x1 - r.y)) << (16 * h);
-      }
-      const int at = n * kHd + (((lane >> 2) ^ (n & 7)) << 4) + (lane & 3) * 4;  // 128-byte swizzle
-      *reinterpret_cast<uint32_t*>(sq + at) = hi;
-      *reinterpret_cast<uint32_t*>(sq + C::kQ + at) = lo;
-      if (lane == 0) {
-        b.unscale[n] = a.scale * kLog2e / up;
-        b.base[n] = 0.f;
-        b.lim[n] = ok ? min(it.key1, paged_key_limit(it.len, it.start + row / G, a.causal_block)) : it.key1;
+        const int k = 64 * h + 32 * ((warp - 8) >> 1) + lane;  // key of the tile
+        const uint8_t* src = smem + C::kOffV + st * kTile + k * kHd;
+        // rows past the range hold anything: their weight is 0, their values must be
+        const bool dead = it.key0 + j * kKeys + k >= it.key1;
+        uint4 u[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          u[c] = *reinterpret_cast<const uint4*>(src + (((4 * half + c) ^ (k & 7)) << 4));
+          if (dead) u[c] = make_uint4(0u, 0u, 0u, 0u);
+        }
+        if (h == 1) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&b.v_empty[st]);
+        }
+        if (j > 0) {  // the previous tile's product of this half has left the buffer
+          ok = __all_sync(0xffffffffu, mbar_wait(&b.pv_done[h], (j - 1) & 1u));
+          if (!ok) break;
+        }
+        uint8_t* dst = sv16 + half * kTile + k * 128;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const uint32_t e[4] = {u[c].x, u[c].y, u[c].z, u[c].w};
+          uint32_t f[8];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            f[2 * i] = f16x2_from_e4m3x2(static_cast<uint16_t>(e[i]));
+            f[2 * i + 1] = f16x2_from_e4m3x2(static_cast<uint16_t>(e[i] >> 16));
+          }
+          *reinterpret_cast<uint4*>(dst + (((2 * c) ^ (k & 7)) << 4)) = make_uint4(f[0], f[1], f[2], f[3]);
+          *reinterpret_cast<uint4*>(dst + (((2 * c + 1) ^ (k & 7)) << 4)) = make_uint4(f[4], f[5], f[6], f[7]);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&b.w_full[h]);
       }
     }
-    fence_proxy_async_smem();
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&b.q_ready);
-    named_sync(2, 128);
+    if (!ok && lane == 0) report_wait(a.err, kErrTimeoutEpilogue, 49, a.total_rows, it.splits);
+  } else if (warp >= 4) {
+    set_registers<kRegsSoftmax, true>();
+    // ---------------- softmax: a key a thread ----------------
+    const int q4 = warp & 3, tid = q4 * 32 + lane;  // TMEM lane
+    const uint32_t lane_base = static_cast<uint32_t>(q4 * 32) << 16;
     // keys from which some row's mask ends (rows are in token order, so the first has the least)
     const int lim_min = b.lim[0];
     const int nc = (it.rows + 15) >> 4;  // 16-column chunks with rows
@@ -334,7 +416,23 @@ __global__ void __launch_bounds__(192, 2)
     for (int j = 0; j < n_tiles; ++j) {
       const int sb = j & 1, st = j % kStages;
       const int key = it.key0 + j * kKeys + tid;
-      ok = ok && mbar_wait(&b.v_full[st], (j / kStages) & 1u) && mbar_wait(&b.s_full[sb], (j >> 1) & 1u);
+      ok = ok && mbar_wait(&b.v_full[st], (j / kStages) & 1u);
+      // x = S (unscale ks) + (log2 vs - base): the pair of every column, once a warp.  Its 32 keys are in one
+      // page, or at page size 16 in two: then the second half's scores and offsets move by the scales' ratios.
+      float inv_vs, ratio = 1.f, shift = 0.f;
+      {
+        __syncwarp();
+        const float2 sc = b.scale[st][tid >> a.page_shift];
+        const bool dead = key >= it.key1;  // (its page may not exist)
+        const float lv = dead ? 0.f : __log2f(sc.y), ks = dead ? 0.f : sc.x;
+        inv_vs = exp2_approx(-lv);
+        const float ks0 = __shfl_sync(0xffffffffu, ks, 0), lv0 = __shfl_sync(0xffffffffu, lv, 0);
+        for (int n = lane; n < nc * 16; n += 32) b.map[q4][n] = make_float2(b.unscale[n] * ks0, lv0 - b.base[n]);
+        if (a.page_shift == 4 && !dead) ratio = ks / ks0, shift = lv - lv0;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&b.v_empty[st]);  // (the scales')
+      }
+      ok = ok && mbar_wait(&b.s_full[sb], (j >> 1) & 1u);
       __syncwarp();
       tc_fence_after_sync();
       float s[N];
@@ -351,36 +449,39 @@ __global__ void __launch_bounds__(192, 2)
       tc_fence_before_sync();
       __syncwarp();
       if (lane == 0) mbar_arrive(&b.s_free[sb]);
-      const float2 sc = b.scale[st][tid >> a.page_shift];
-      const bool dead = key >= it.key1;
-      const float lv = dead ? 0.f : __log2f(sc.y), inv_vs = exp2_approx(-lv), ks = dead ? 0.f : sc.x;
-      float top = -INFINITY;
+      float top0 = -INFINITY, top1 = -INFINITY;
+      const float4* map = reinterpret_cast<const float4*>(b.map[q4]);
+      const bool edge = it.key0 + (j + 1) * kKeys > lim_min;
 #pragma unroll
       for (int c = 0; c < N / 16; ++c) {
         if (c < nc) {
+          float4 m[8];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int n = c * 16 + i;
-            s[n] = dead ? -INFINITY : fmaf(s[n], b.unscale[n] * ks, lv - b.base[n]);
+          for (int i = 0; i < 8; ++i) m[i] = map[c * 8 + i];
+          if (a.page_shift == 4) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[c * 16 + i] *= ratio;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) m[i].y += shift, m[i].w += shift;
           }
-        }
-      }
-      if (it.key0 + (j + 1) * kKeys > lim_min) {
 #pragma unroll
-        for (int c = 0; c < N / 16; ++c)
-          if (c < nc) {
+          for (int i = 0; i < 8; ++i) {
+            s[c * 16 + 2 * i] = fmaf(s[c * 16 + 2 * i], m[i].x, m[i].y);
+            s[c * 16 + 2 * i + 1] = fmaf(s[c * 16 + 2 * i + 1], m[i].z, m[i].w);
+          }
+          if (edge) {
 #pragma unroll
             for (int i = 0; i < 16; ++i)
-              if (key >= b.lim[c * 16 + i]) s[c * 16 + i] = -INFINITY;
+              if (key >= b.lim[c * 16 + i]) s[c * 16 + i] = -INFINITY;  // (also what a dead key's garbage gave)
           }
-      }
 #pragma unroll
-      for (int c = 0; c < N / 16; ++c)
-        if (c < nc) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) top = fmaxf(top, s[c * 16 + i]);
+          for (int i = 0; i < 16; i += 2) {
+            top0 = fmaxf(top0, s[c * 16 + i]);
+            top1 = fmaxf(top1, s[c * 16 + i + 1]);
+          }
         }
-      if (any_of_128(top > kTrip || j == 0 || !ok)) {
+      }
+      if (any_of_128(fmaxf(top0, top1) > kTrip || j == 0 || !ok)) {
         if (any_of_128(!ok)) {  // a wait expired: all four warps leave together
           ok = false;
           break;
@@ -406,7 +507,7 @@ __global__ void __launch_bounds__(192, 2)
         }
         named_sync(2, 128);
         if (j > 0) {  // O of the earlier tiles: their last product has to land first
-          ok = mbar_wait(&b.pv_done, (j - 1) & 1u);
+          ok = mbar_wait(&b.pv_done[1], (j - 1) & 1u);
           __syncwarp();
           tc_fence_after_sync();
 #pragma unroll 1
@@ -446,34 +547,9 @@ __global__ void __launch_bounds__(192, 2)
         }
         *reinterpret_cast<uint4*>(p + c * (kKeys * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
       }
-      // V_j in f16: this key's row, once P_{j-1} V_{j-1} has left the tile.  Rows past the range hold anything:
-      // their weight is 0, their values must be.
-      if (j > 0) ok = ok && mbar_wait(&b.pv_done, (j - 1) & 1u);
-      {
-        const uint8_t* src = smem + C::kOffV + st * kTile + tid * kHd;
-#pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          uint4 u = make_uint4(0u, 0u, 0u, 0u);
-          if (!dead) u = *reinterpret_cast<const uint4*>(src + ((c ^ (tid & 7)) << 4));
-          const uint32_t e[4] = {u.x, u.y, u.z, u.w};
-          uint32_t f[8];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            f[2 * i] = f16x2_from_e4m3x2(static_cast<uint16_t>(e[i]));
-            f[2 * i + 1] = f16x2_from_e4m3x2(static_cast<uint16_t>(e[i] >> 16));
-          }
-          // columns 16 c ..: 16-byte units 2 c and 2 c + 1 of the row, eight a sub-tile
-          uint8_t* dst = sv16 + (c >> 2) * kTile + tid * 128;
-          *reinterpret_cast<uint4*>(dst + (((2 * c & 7) ^ (tid & 7)) << 4)) = make_uint4(f[0], f[1], f[2], f[3]);
-          *reinterpret_cast<uint4*>(dst + (((2 * c + 1 & 7) ^ (tid & 7)) << 4)) = make_uint4(f[4], f[5], f[6], f[7]);
-        }
-      }
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(&b.v_empty[st]);
-        mbar_arrive(&b.p_full);
-      }
+      if (lane == 0) mbar_arrive(&b.p_full);
     }
 
     // row sums over the 128 keys: lane l of a warp ends with column l & 15 of each 16-column chunk
@@ -505,13 +581,9 @@ __global__ void __launch_bounds__(192, 2)
     }
     named_sync(2, 128);
     tc_fence_after_sync();
-    // O^T: lane = head column, a row a TMEM column
-    bf16* out = static_cast<bf16*>(a.out);
-    float* part = reinterpret_cast<float*>(a.part + it.part);  // this item's partial: [N][128], then [N] (base, sum)
-    auto out_row = [&](int n) {
-      const int row = it.row0 + n;
-      return out + (static_cast<size_t>(it.tok0 + row / G) * a.hq + it.head * G + row % G) * kHd;
-    };
+    // O^T: lane = head column, a row a TMEM column.  A split tile leaves its partial: [N][128], then [N] (base, sum)
+    bf16* out = static_cast<bf16*>(a.out) + tid;
+    float* part = reinterpret_cast<float*>(a.part + it.part) + tid;
 #pragma unroll 1
     for (int c = 0; c < nc; ++c) {
       uint32_t v[16];
@@ -522,61 +594,79 @@ __global__ void __launch_bounds__(192, 2)
         const int n = c * 16 + i;
         if (n >= it.rows) continue;
         const float x = __uint_as_float(v[i]) * b.factor[n];
-        if (it.splits == 1) out_row(n)[tid] = __float2bfloat16_rn(x);
-        else part[n * kHd + tid] = x;
+        if (it.splits == 1) out[static_cast<size_t>(b.out[n]) * kHd] = __float2bfloat16_rn(x);
+        else part[n * kHd] = x;
       }
     }
     if (it.splits > 1) {
-      if (tid < it.rows) reinterpret_cast<float2*>(part + N * kHd)[tid] = make_float2(b.base[tid], b.delta[tid]);
+      if (tid < it.rows)
+        reinterpret_cast<float2*>(reinterpret_cast<float*>(a.part + it.part) + N * kHd)[tid] = make_float2(b.base[tid], b.delta[tid]);
       __threadfence();
-      named_sync(2, 128);
-      if (tid == 0) b.last = atomicAdd(&a.arrived[it.tile], 1u) == static_cast<unsigned>(it.splits - 1);
-      named_sync(2, 128);
-      if (b.last) {  // the tile's last item adds the partials
-        __threadfence();
-        constexpr int kPart = N * kHd + 4 * N;  // floats
-        const float* first = part - static_cast<size_t>(it.split) * kPart;
-        for (int n = q4; n < it.rows; n += 4) {  // a warp a row, four columns a lane
-          float m = -INFINITY;
-          for (int s = 0; s < it.splits; ++s) {
-            const float2 bs = __ldcg(reinterpret_cast<const float2*>(first + s * kPart + N * kHd) + n);
-            if (bs.y != 0.f) m = fmaxf(m, bs.x);
-          }
-          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-          float l = 0.f;
-#pragma unroll 8
-          for (int s = 0; s < it.splits; ++s) {
-            const float2 bs = __ldcg(reinterpret_cast<const float2*>(first + s * kPart + N * kHd) + n);
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(first + s * kPart + n * kHd) + lane);
-            const float f = bs.y != 0.f ? exp2f(bs.x - m) : 0.f;
-            l += f * bs.y;
-            acc.x += f * v.x, acc.y += f * v.y, acc.z += f * v.z, acc.w += f * v.w;
-          }
-          const float inv = l != 0.f ? 1.f / l : 0.f;
-          *reinterpret_cast<uint2*>(out_row(n) + 4 * lane) =
-              make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
-        }
-        if (tid == 0) a.arrived[it.tile] = 0;  // ready for the next call
-      }
     }
     tc_fence_before_sync();
   }
   __syncwarp();
   tc_fence_before_sync();
   __syncthreads();
+  // Back to the launch's split.  Only here, past the barrier: a warp without a role that took its registers
+  // back any earlier would leave the softmax waiting for them.
+  if (warp >= 4 && warp < 8) set_registers<kRegsLaunch, false>();
+  else set_registers<kRegsLaunch, true>();
   if (warp == 1) {
     tc_fence_after_sync();
     tmem_dealloc(tmem, C::kCols);
   }
+  if (it.splits == 1) return;
+
+  // the tile's last item adds the partials, all threads: a row's weights 2^(base - max) / sum, then its columns
+  if (threadIdx.x == 0) b.last = atomicAdd(&a.arrived[it.tile], 1u) == static_cast<unsigned>(it.splits - 1);
+  __syncthreads();
+  if (!b.last) return;
+  __threadfence();
+  constexpr int kPart = N * kHd + 4 * N;  // floats
+  const float* first = reinterpret_cast<const float*>(a.part + it.part) - static_cast<size_t>(it.split) * kPart;
+  float* weight = reinterpret_cast<float*>(smem);  // [kMaxPagedSplits][N], over the K ring
+  for (int n = warp; n < it.rows; n += kThreads / 32) {  // a lane a split
+    float2 bs = make_float2(0.f, 0.f);
+    if (lane < it.splits) bs = __ldcg(reinterpret_cast<const float2*>(first + lane * kPart + N * kHd) + n);
+    float m = bs.y != 0.f ? bs.x : -INFINITY;
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+    const float f = bs.y != 0.f ? exp2f(bs.x - m) : 0.f;
+    float l = f * bs.y;
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+    weight[lane * N + n] = l != 0.f ? f / l : 0.f;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < it.rows * (kHd / 4); i += kThreads) {
+    const int n = i >> 5, c4 = i & 31;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+    for (int s = 0; s < it.splits; ++s) {
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(first + s * kPart + n * kHd) + c4);
+      const float f = weight[s * N + n];
+      acc.x += f * v.x, acc.y += f * v.y, acc.z += f * v.z, acc.w += f * v.w;
+    }
+    *reinterpret_cast<uint2*>(static_cast<bf16*>(a.out) + static_cast<size_t>(b.out[n]) * kHd + 4 * c4) =
+        make_uint2(pack_bf16x2(acc.x, acc.y), pack_bf16x2(acc.z, acc.w));
+  }
+  if (threadIdx.x == 0) a.arrived[it.tile] = 0;  // ready for the next call
 }
 
 template <int N>
 static int launch_n(const PagedAttnArgs& a, int n_items, const CUtensorMap& k, const CUtensorMap& v, cudaStream_t s) {
-  return launch_k(paged_attn_tc_kernel<N>, dim3(n_items), dim3(192), Cfg<N>::kBytes, s, a, k, v);
+  return launch_k(paged_attn_tc_kernel<N>, dim3(n_items), dim3(kThreads), Cfg<N>::kBytes, s, a, k, v);
 }
+// The register split only ever asks for what the launch brought: checked here, not by waiting for more.
 template <int N>
 static cudaError_t opt_in() {
-  return cudaFuncSetAttribute(paged_attn_tc_kernel<N>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<N>::kBytes);
+  cudaFuncAttributes f;
+  cudaError_t e = cudaFuncGetAttributes(&f, paged_attn_tc_kernel<N>);
+  if (e == cudaSuccess && f.numRegs < kRegsLaunch) e = cudaErrorInvalidKernelImage;
+  return e != cudaSuccess ? e
+                          : cudaFuncSetAttribute(paged_attn_tc_kernel<N>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                 Cfg<N>::kBytes);
 }
 
 int init_paged_attention_tc_attributes() {
