@@ -111,13 +111,24 @@ __device__ __forceinline__ bool any_of_256(bool p) {
   return r != 0;
 }
 
-// Order-preserving map of floats to unsigned ints (for the integer warp reductions).
-__device__ __forceinline__ uint32_t ordered(float x) {
-  const uint32_t b = __float_as_uint(x);
-  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
-}
-__device__ __forceinline__ float unordered(uint32_t r) {
-  return __uint_as_float((r & 0x80000000u) ? (r & 0x7FFFFFFFu) : ~r);
+// Eight values a lane, combined over the warp's 32 lanes (f: max or plus): lane l ends with value l & 7.  Halves
+// of the values change hands at each of three steps, so it takes 9 shuffles, not 40.
+template <typename F>
+__device__ __forceinline__ float reduce_columns(const float* x, int lane, F f) {
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = x[i];
+#pragma unroll
+  for (int h = 4; h >= 1; h >>= 1) {
+    const bool up = (lane & h) != 0;
+#pragma unroll
+    for (int i = 0; i < h; ++i) {
+      const float keep = up ? v[i + h] : v[i], give = up ? v[i] : v[i + h];
+      v[i] = f(keep, __shfl_xor_sync(0xffffffffu, give, h));
+    }
+  }
+  v[0] = f(v[0], __shfl_xor_sync(0xffffffffu, v[0], 8));
+  return f(v[0], __shfl_xor_sync(0xffffffffu, v[0], 16));
 }
 
 constexpr int kThreads = 384;
@@ -340,7 +351,8 @@ __global__ void __launch_bounds__(kThreads, 2)
         const float x[4] = {__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xFFFF0000u), __uint_as_float(u.y << 16),
                             __uint_as_float(u.y & 0xFFFF0000u)};
         float m = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
-        m = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m)));
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
         // exponent of m, kept where both the scale and its inverse are normal floats
         const int e = min(max(static_cast<int>(__float_as_uint(m) >> 23) - 127, -110), 110);
         const float up = m > 0.f ? __uint_as_float(static_cast<uint32_t>(127 + 7 - e) << 23) : 1.f;
@@ -376,7 +388,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     const uint32_t lane_base = (static_cast<uint32_t>(q4 * 32) << 16) + col0;
     // keys from which some row's mask ends (rows are in token order, so the first has the least)
     const int lim_min = b.lim[0];
-    const int nc = min(max(it.rows - col0 + 7, 0) >> 3, H / 8);  // 8-column chunks with rows
+    const bool mine = it.rows > col0;  // rows among this warpgroup's columns
     float sum[H];
 #pragma unroll
     for (int n = 0; n < H; ++n) sum[n] = 0.f;
@@ -390,50 +402,52 @@ __global__ void __launch_bounds__(kThreads, 2)
       ok = ok && mbar_wait(&b.s_full, j & 1u);
       __syncwarp();
       tc_fence_after_sync();
-      float s[H];
+      // (no branch on the number of rows between here and the store of P: straight-line code hides the latencies)
+      float s[H], top0 = -INFINITY, top1 = -INFINITY;
+      if (mine) {
+        uint32_t hi[H / 8][8], lo[H / 8][8];
 #pragma unroll
-      for (int c = 0; c < H / 8; ++c) {
-        if (c < nc) {
-          uint32_t hi[8], lo[8];
-          tmem_ld_32x32b_x8(tmem + lane_base + C::kS + c * 8, hi);
-          tmem_ld_32x32b_x8(tmem + lane_base + C::kS + N + c * 8, lo);
-          tmem_ld_wait();
-          after_wait(hi);
-          after_wait(lo);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) s[c * 8 + i] = __uint_as_float(hi[i]) + __uint_as_float(lo[i]);
+        for (int c = 0; c < H / 8; ++c) {
+          tmem_ld_32x32b_x8(tmem + lane_base + C::kS + c * 8, hi[c]);
+          tmem_ld_32x32b_x8(tmem + lane_base + C::kS + N + c * 8, lo[c]);
         }
+        tmem_ld_wait();
+#pragma unroll
+        for (int c = 0; c < H / 8; ++c) {
+          after_wait(hi[c]);
+          after_wait(lo[c]);
+        }
+#pragma unroll
+        for (int n = 0; n < H; ++n) s[n] = __uint_as_float(hi[n / 8][n % 8]) + __uint_as_float(lo[n / 8][n % 8]);
       }
       tc_fence_before_sync();
       __syncwarp();
       if (lane == 0) mbar_arrive(&b.s_free);
-      float top0 = -INFINITY, top1 = -INFINITY;
-      const float4* map = reinterpret_cast<const float4*>(&b.map[st][q4][col0]);
-      const float4* base = reinterpret_cast<const float4*>(&b.base[col0]);
-      const bool edge = it.key0 + (j + 1) * kKeys > lim_min;
+      if (mine) {
+        const float4* map = reinterpret_cast<const float4*>(&b.map[st][q4][col0]);
+        const float4* base = reinterpret_cast<const float4*>(&b.base[col0]);
+        if (a.page_shift == 4) {
 #pragma unroll
-      for (int c = 0; c < H / 8; ++c) {
-        if (c < nc) {
+          for (int n = 0; n < H; ++n) s[n] *= sc.z;
+        }
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const float4 m = map[c * 2 + i], bs = base[c * 2 + i];
-            float* x = &s[c * 8 + 4 * i];
-            if (a.page_shift == 4) x[0] *= sc.z, x[1] *= sc.z, x[2] *= sc.z, x[3] *= sc.z;
-            x[0] = fmaf(x[0], m.x, sc.x - bs.x);
-            x[1] = fmaf(x[1], m.y, sc.x - bs.y);
-            x[2] = fmaf(x[2], m.z, sc.x - bs.z);
-            x[3] = fmaf(x[3], m.w, sc.x - bs.w);
-          }
-          if (edge) {
+        for (int i = 0; i < H / 4; ++i) {
+          const float4 m = map[i], bs = base[i];
+          float* x = &s[4 * i];
+          x[0] = fmaf(x[0], m.x, sc.x - bs.x);
+          x[1] = fmaf(x[1], m.y, sc.x - bs.y);
+          x[2] = fmaf(x[2], m.z, sc.x - bs.z);
+          x[3] = fmaf(x[3], m.w, sc.x - bs.w);
+        }
+        if (it.key0 + (j + 1) * kKeys > lim_min) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-              if (key >= b.lim[col0 + c * 8 + i]) s[c * 8 + i] = -INFINITY;  // (also what a dead key's garbage gave)
-          }
+          for (int n = 0; n < H; ++n)
+            if (key >= b.lim[col0 + n]) s[n] = -INFINITY;  // (also what a dead key's garbage gave)
+        }
 #pragma unroll
-          for (int i = 0; i < 8; i += 2) {
-            top0 = fmaxf(top0, s[c * 8 + i]);
-            top1 = fmaxf(top1, s[c * 8 + i + 1]);
-          }
+        for (int n = 0; n < H; n += 2) {
+          top0 = fmaxf(top0, s[n]);
+          top1 = fmaxf(top1, s[n + 1]);
         }
       }
       if (any_of_256(fmaxf(top0, top1) > kTrip || j == 0 || !ok)) {
@@ -442,15 +456,13 @@ __global__ void __launch_bounds__(kThreads, 2)
           break;
         }
         // move the bases of the columns that need it to their maximum over these 128 keys
+        if (mine) {
 #pragma unroll
-        for (int c = 0; c < H / 8; ++c)
-          if (c < nc) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const uint32_t m = __reduce_max_sync(0xffffffffu, ordered(s[c * 8 + i]));
-              if (lane == 0) b.part[q4][col0 + c * 8 + i] = unordered(m);
-            }
+          for (int c = 0; c < H / 8; ++c) {
+            const float m = reduce_columns(&s[c * 8], lane, [](float x, float y) { return fmaxf(x, y); });
+            if (lane < 8) b.part[q4][col0 + c * 8 + lane] = m;
           }
+        }
         named_sync(2, 256);
         const int t = threadIdx.x - 128;
         if (t < N) {
@@ -467,7 +479,7 @@ __global__ void __launch_bounds__(kThreads, 2)
           __syncwarp();
           tc_fence_after_sync();
 #pragma unroll 1
-          for (int c = 0; c < nc; ++c) {
+          for (int c = 0; c < (mine ? H / 8 : 0); ++c) {
 #pragma unroll 1
             for (int term = 0; term < 3; ++term) {
               uint32_t v[8];
@@ -483,9 +495,9 @@ __global__ void __launch_bounds__(kThreads, 2)
           tmem_st_wait();
           tc_fence_before_sync();
         }
+        if (mine) {
 #pragma unroll
-        for (int n = 0; n < H; ++n) {
-          if (n < nc * 8) {
+          for (int n = 0; n < H; ++n) {
             s[n] += b.delta[col0 + n];
             if (j > 0) sum[n] *= b.factor[col0 + n];
           }
@@ -494,9 +506,9 @@ __global__ void __launch_bounds__(kThreads, 2)
       // P_j: with two buffers P_{j-2} has left this one (S_j's commit covered every product issued before it)
       if (C::kPBufs == 1 && j > 0) ok = ok && mbar_wait(&b.pv_done[(j - 1) & 1], ((j - 1) >> 1) & 1u);
       uint8_t* p = smem + C::kOffP + (j % C::kPBufs) * C::kP + key_lane * 16;
+      if (mine) {
 #pragma unroll
       for (int c = 0; c < H / 8; ++c) {
-        if (c >= nc) continue;
         uint32_t w[3][2];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -519,6 +531,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         for (int term = 0; term < 3; ++term)
           *reinterpret_cast<uint2*>(p + (term * (N / 16) + (col >> 4)) * C::kUnit + (col & 8)) = make_uint2(w[term][0], w[term][1]);
       }
+      }
       if (key >= it.key1) {  // rows past the range hold anything: their weight is 0, their values must be
         uint4* v = reinterpret_cast<uint4*>(smem + C::kOffV + st * kTile + key_lane * kHd) + (col0 == 0 ? 0 : 4);
 #pragma unroll
@@ -529,25 +542,13 @@ __global__ void __launch_bounds__(kThreads, 2)
       if (lane == 0) mbar_arrive(&b.p_full);
     }
 
-    // row sums over the 128 keys: lane l of a warp ends with column l & 7 of each 8-column chunk
+    // row sums over the 128 keys
+    if (mine) {
 #pragma unroll
-    for (int c = 0; c < H / 8; ++c) {
-      if (c >= nc) continue;
-      float v[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = sum[c * 8 + i];
-#pragma unroll
-      for (int h = 4; h >= 1; h >>= 1) {
-        const bool up = (lane & h) != 0;
-#pragma unroll
-        for (int i = 0; i < h; ++i) {
-          const float keep = up ? v[i + h] : v[i], give = up ? v[i] : v[i + h];
-          v[i] = keep + __shfl_xor_sync(0xffffffffu, give, h);
-        }
+      for (int c = 0; c < H / 8; ++c) {
+        const float l = reduce_columns(&sum[c * 8], lane, [](float x, float y) { return x + y; });
+        if (lane < 8) b.part[q4][col0 + c * 8 + lane] = l;
       }
-      v[0] += __shfl_xor_sync(0xffffffffu, v[0], 8);
-      v[0] += __shfl_xor_sync(0xffffffffu, v[0], 16);
-      if (lane < 8) b.part[q4][col0 + c * 8 + lane] = v[0];
     }
     ok = __all_sync(0xffffffffu, ok && mbar_wait(&b.o_final, 0));
     if (!ok && lane == 0) report_wait(a.err, kErrTimeoutEpilogue, 46, a.total_rows, it.splits);
@@ -563,22 +564,30 @@ __global__ void __launch_bounds__(kThreads, 2)
     // O^T: lane = head column, a row a TMEM column.  A split tile leaves its partial: [N][128], then [N] (base, sum)
     bf16* out = static_cast<bf16*>(a.out) + key_lane;
     float* part = reinterpret_cast<float*>(a.part + it.part) + key_lane;
-#pragma unroll 1
-    for (int c = 0; c < nc; ++c) {
-      uint32_t v[3][8];
+    if (mine) {
 #pragma unroll
-      for (int term = 0; term < 3; ++term) tmem_ld_32x32b_x8(tmem + lane_base + C::kO + term * N + c * 8, v[term]);
-      tmem_ld_wait();
+      for (int c = 0; c < H / 8; ++c) {
+        uint32_t v[3][8];
 #pragma unroll
-      for (int term = 0; term < 3; ++term) after_wait(v[term]);
+        for (int term = 0; term < 3; ++term) tmem_ld_32x32b_x8(tmem + lane_base + C::kO + term * N + c * 8, v[term]);
+        tmem_ld_wait();
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int n = col0 + c * 8 + i;
-        if (n >= it.rows) continue;
-        const float x = (__uint_as_float(v[0][i]) + (__uint_as_float(v[1][i]) + __uint_as_float(v[2][i]) * 0.03125f) * 0.03125f) *
-                        b.factor[n];
-        if (it.splits == 1) out[static_cast<size_t>(b.out[n]) * kHd] = __float2bfloat16_rn(x);
-        else part[n * kHd] = x;
+        for (int term = 0; term < 3; ++term) after_wait(v[term]);
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          x[i] = (__uint_as_float(v[0][i]) + (__uint_as_float(v[1][i]) + __uint_as_float(v[2][i]) * 0.03125f) * 0.03125f) *
+                 b.factor[col0 + c * 8 + i];
+        const int n0 = col0 + c * 8;
+        if (it.splits == 1) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (n0 + i < it.rows) out[static_cast<size_t>(b.out[n0 + i]) * kHd] = __float2bfloat16_rn(x[i]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (n0 + i < it.rows) part[(n0 + i) * kHd] = x[i];
+        }
       }
     }
     if (it.splits > 1) {
