@@ -91,9 +91,11 @@ int plan_items(const fdllm_handle* h, const std::vector<PagedReq>& reqs, int cau
   const fdllm_config& c = h->cfg;
   const int G = c.num_attention_heads / c.num_key_value_heads, heads = c.num_key_value_heads;
   const bool tc = c.head_dim == 128;
-  const int unit = tc ? 16 : 8, largest = tc ? 48 : 24;
+  const int unit = tc ? 16 : 8, narrow = tc ? 48 : 24;  // largest tile of the classes by rows
+  auto is_wide = [&](long long rows) { return tc && rows > narrow; };
   const long long slots = (tc ? 2LL : 3LL) * h->num_sms;
   auto tile_rows = [&](long long rows) {
+    const int largest = is_wide(rows) ? 128 : narrow;
     const long long tiles = (rows + largest - 1) / largest;
     return static_cast<int>(((rows + tiles - 1) / tiles + unit - 1) / unit * unit);
   };
@@ -124,13 +126,14 @@ int plan_items(const fdllm_handle* h, const std::vector<PagedReq>& reqs, int cau
     const PagedReq& r = reqs[i];
     const long long rows = static_cast<long long>(r.rows) * G;
     if (rows == 0) continue;
-    const int step = tile_rows(rows), cls = step / unit - 1;
+    const int step = tile_rows(rows), cls = is_wide(rows) ? kPagedWide : step / unit - 1;
+    const int part_rows = is_wide(rows) ? 128 : step;
     for (long long t = 0; t < rows; t += step) {
       const int keys = keys_of(r, std::min(rows, t + step));
       const int want = splits_of(keys, share);
       const int each = ((keys + want - 1) / want + kShareUnit - 1) / kShareUnit * kShareUnit;
       const int splits = (keys + each - 1) / each;
-      const int part = step * (c.head_dim / 4) + step;  // 16-byte units
+      const int part = part_rows * (c.head_dim / 4) + part_rows;  // 16-byte units
       for (int head = 0; head < heads; ++head) {
         for (int s = 0; s < splits; ++s) {
           PagedItem it{};
@@ -343,8 +346,9 @@ int fdllm_paged_attention(fdllm_handle* h, const fdllm_paged_cache* cache, int l
       if (plan->priv[kPagedItems + k] == 0) continue;
       a.items = reinterpret_cast<const PagedItem*>(plan_words + plan->priv[kPagedItemOff + k]);
       const int n = plan->priv[kPagedItems + k];
-      CUDA_TRY(c.head_dim == 128 ? launch_paged_attention_tc(a, 16 * (k + 1), n, tm_k, tm_v, st)
-                                 : launch_paged_attention_narrow(a, k + 1, n, tm_k, tm_v, st));
+      CUDA_TRY(c.head_dim != 128  ? launch_paged_attention_narrow(a, k + 1, n, tm_k, tm_v, st)
+               : k == kPagedWide ? launch_paged_attention_wide(a, n, tm_k, tm_v, st)
+                                 : launch_paged_attention_tc(a, 16 * (k + 1), n, tm_k, tm_v, st));
     }
     return FDLLM_OK;
   });

@@ -46,9 +46,10 @@ struct alignas(16) PagedItem {
 };
 static_assert(sizeof(PagedItem) == 4 * kPagedItemWords, "plan item layout");
 
-// Item classes, a launch each: tiles of 16, 32 and 48 query rows at head_dim 128 (tcgen05), of 8, 16 and 24 at
-// the others (mma.sync).
-constexpr int kPagedClasses = 3;
+// Item classes, a launch each: tiles of 16, 32 and 48 query rows (keys on the MMA's M side) and of up to 128 (rows
+// on it) at head_dim 128, of 8, 16 and 24 at the others (mma.sync).
+constexpr int kPagedClasses = 4;
+constexpr int kPagedWide = 3;
 
 // fdllm_paged_plan::priv
 enum PagedPriv : int {
@@ -123,6 +124,8 @@ int launch_paged_attention_narrow(const PagedAttnArgs& a, int nt, int n_items, c
                                   cudaStream_t s);
 int launch_paged_attention_tc(const PagedAttnArgs& a, int cols, int n_items, const CUtensorMap& k, const CUtensorMap& v,
                               cudaStream_t s);
+int launch_paged_attention_wide(const PagedAttnArgs& a, int n_items, const CUtensorMap& k, const CUtensorMap& v,
+                                cudaStream_t s);
 // CTAs a row is split into, and chunks each.
 int logprobs_parts(int rows, int vocab, int dtype, int num_sms, int* part_chunks);
 int launch_logprobs(const LogprobArgs& a, int dtype, int parts, int part_chunks, cudaStream_t s);

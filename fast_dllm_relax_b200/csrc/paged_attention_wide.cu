@@ -1,0 +1,521 @@
+// Attention over a paged 8-bit KV cache on the 5th-generation tensor cores for many query rows
+// (fdllm_paged_attention, bf16, head_dim 128): block steps and prompts.  Semantics as in paged_attention.cu.
+//
+// The query rows of one request and KV head are its (token, query head) pairs.  A CTA takes one item of the
+// plan, a tile of at most 128 rows and a range of keys, in tiles of 64 keys with the rows on the MMA's M side:
+//   S [128, 64]   = (Qh + Ql) K^T     A: the queries (e4m3 in shared memory), B: the K tile as cached (e4m3)
+//   P [128, 64]   = 2^(a S + log2 vs - B)
+//   O [128, 128] += P V               A: P (f16 in TMEM, over its S), B: V widened to f16 (exact)
+// Precision: a bf16 query has 8 significant bits, so Q = Qh + Ql under one power of two per row (largest element
+// in [2^7, 2^8)) is exact for elements above 2^-10 of the row's largest and to 2^-18 of it below; two 8-bit
+// products cost one 16-bit product's time and K needs no widening.  P keeps 11 bits and weights down to 2^-32 of
+// the largest.  A row's base B moves only when a weight passes 2^kTrip (then its maximum sits at 2^kSeat); then
+// its row of O in TMEM is scaled.  log2 vs in the exponent keeps P in range whatever the page scales are; the row
+// sum takes it back out.
+//
+// Roles (384 threads, registers moved to the softmax): warp 0 the TMA producer (a lane a page; page ids and
+// scales 32 pages at a time), warp 1 the MMA issuer and TMEM owner, warps 4-7 the softmax, a row a thread,
+// warps 8-11 widen V.  S, P and the widened V are double-buffered: S_{j+1} and V_{j+1} are made while tile j is
+// in the softmax.  Two CTAs share an SM (256 TMEM columns and 97 KB each), so one's softmax covers the other's
+// products.
+//
+// What bounds it: shared-memory traffic, about 104 KB a tile of 8192 scores (Q twice 16 KB and K twice 8 KB for S,
+// 24 KB to widen V and 16 KB to use it, 16 KB of copies), 812 clocks at 128 bytes a clock; the exponentials of two
+// CTAs come next (512 clocks each).
+//
+// A tile whose keys are split over several items joins them through the workspace as in
+// paged_attention_narrow.cu: the last item to arrive adds the partials in item order.
+#include "paged.h"
+
+namespace fdllm {
+
+namespace {
+
+constexpr int kRows = 128, kKeys = 64, kHd = 128;
+constexpr int kTile = kKeys * kHd;      // bytes of a K or V tile as cached
+constexpr int kQ = kRows * kHd;         // bytes of Qh or Ql
+constexpr int kV16 = kKeys * kHd * 2;   // bytes of a widened V tile: two sub-tiles of 64 columns
+constexpr int kOffQ = 0, kOffK = 2 * kQ, kOffV = kOffK + 2 * kTile, kOffV16 = kOffV + 2 * kTile;
+constexpr int kBytes = 1024 + kOffV16 + 2 * kV16;
+constexpr uint32_t kTmemS = 0, kTmemO = 128, kTmemCols = 256;  // S: two buffers of 64 columns
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kTrip = 15.f, kSeat = 8.f;
+constexpr int kThreads = 384;
+constexpr int kRegsLaunch = 80, kRegsMisc = 48, kRegsSoftmax = 144, kRegsWiden = 48;
+static_assert(kRegsMisc + kRegsSoftmax + kRegsWiden == 3 * kRegsLaunch, "the split is the launch's registers");
+static_assert(2 * (kBytes + 2048) <= 228 * 1024, "two CTAs per SM");
+
+// Instruction descriptors, fp32 accumulator, M 128: S (kind::f8f6f4, e4m3, K-major) and O (kind::f16, f16, A in
+// TMEM, B MN-major).
+constexpr uint32_t kIdescS = (1u << 4) | ((kKeys >> 3) << 17) | ((128u >> 4) << 24);
+constexpr uint32_t kIdescO = (1u << 4) | (1u << 16) | ((kHd >> 3) << 17) | ((128u >> 4) << 24);
+
+__device__ __forceinline__ void mma_f8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// D[tmem] (+)= A[tmem] * B[smem]^T, f16 operands (two to a TMEM column of A).
+__device__ __forceinline__ void mma_f16_ta(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+__device__ __forceinline__ void after_wait(uint32_t (&r)[32]) {  // a load's registers are read only after its wait
+#pragma unroll
+  for (int i = 0; i < 32; ++i) asm volatile("" : "+r"(r[i]));
+}
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+template <int kRegs, bool kGrow>
+__device__ __forceinline__ void set_registers() {
+  if constexpr (kGrow) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs));
+  else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs));
+}
+
+struct Bars {
+  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
+  uint64_t scale_full[4], q_ready, s_full[2], p_full[2], w_full[2], pv_done[2], o_final;
+  uint32_t tmem;
+  int last;
+  float4 scale[4][kKeys / 16];  // of tile j & 3, its 16-key groups: ks, log2 vs, 1 / vs
+};
+
+}  // namespace
+
+__global__ void __launch_bounds__(kThreads, 2)
+    paged_attn_wide_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap tm_k,
+                           const __grid_constant__ CUtensorMap tm_v) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  __shared__ Bars b;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&b.k_full[i], 32);
+      mbar_init(&b.k_empty[i], 1);
+      mbar_init(&b.v_full[i], 32);
+      mbar_init(&b.v_empty[i], 4);
+      mbar_init(&b.s_full[i], 1);
+      mbar_init(&b.p_full[i], 4);
+      mbar_init(&b.w_full[i], 4);
+      mbar_init(&b.pv_done[i], 1);
+    }
+    for (int i = 0; i < 4; ++i) mbar_init(&b.scale_full[i], 1);
+    mbar_init(&b.q_ready, 4);
+    mbar_init(&b.o_final, 1);
+    mbar_fence_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(&b.tmem, kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = b.tmem;
+  pdl_trigger();
+  pdl_wait();
+  const PagedItem it = a.items[blockIdx.x];
+  const int G = a.hq / a.hkv;
+  const int n_tiles = (it.key1 - it.key0 + kKeys - 1) / kKeys;
+
+  if (warp < 4) set_registers<kRegsMisc, false>();
+  if (warp == 0) {
+    // ---------------- TMA producer: a lane a page ----------------
+    const int ps = a.page_size, per_tile = max(kKeys >> a.page_shift, 1), box = min(ps, kKeys);
+    const int* table = a.table + static_cast<size_t>(it.req) * a.table_ld;
+    const uint64_t policy = l2_policy_evict_last();  // the other tiles of this request read them too
+    int batch = -32, row = 0;  // first page of the 32 whose rows and scales the lanes hold
+    float ks = 1.f, vs = 1.f;
+    int issued = 0;
+    for (int j = 0; j < n_tiles; ++j, ++issued) {
+      const int key = it.key0 + j * kKeys, page0 = key >> a.page_shift, st = j & 1;
+      if (page0 + per_tile > batch + 32) {  // uniform
+        batch = page0;
+        const int p = page0 + lane;
+        if (static_cast<long long>(p) * ps < it.key1) {
+          const int id = max(paged_page_id(table[p], a.pages, a.err), 0);
+          const size_t unit = static_cast<size_t>(id) * a.hkv + it.head;
+          row = static_cast<int>(unit << a.page_shift);
+          ks = __ldg(a.k_scale + unit);
+          vs = __ldg(a.v_scale + unit);
+        }
+      }
+      const int from = page0 - batch + (lane < per_tile ? lane : 0);
+      const int src = a.layer_row + __shfl_sync(0xffffffffu, row, from) + (key & (ps - 1));  // (half of a page of 128)
+      const bool live = lane < per_tile && static_cast<long long>(page0 + lane) * ps < it.key1;
+      const uint32_t free_parity = ((j >> 1) & 1u) ^ 1u;
+      auto load = [&](const CUtensorMap* map, uint64_t* bar, uint8_t* dst) {
+        asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_addr(bar)), "r"(box * kHd)
+                     : "memory");
+        tma_load_2d(dst + lane * box * kHd, map, bar, 0, src, policy);
+      };
+      if (!__all_sync(0xffffffffu, mbar_wait(&b.k_empty[st], free_parity))) {
+        report_wait(a.err, kErrTimeoutProducer, 51, a.total_rows, it.splits);
+        break;
+      }
+      if (live) load(&tm_k, &b.k_full[st], smem + kOffK + st * kTile);
+      // the scales of the tile's 16-key groups.  Slot j & 3: S_{j-2} is done, so P_{j-4} is used and its softmax past.
+      // A barrier of their own: K's may be two phases on before the softmax comes to this tile.
+      const int group_page = page0 - batch + ((16 * (lane & 3)) >> a.page_shift);
+      const float kg = __shfl_sync(0xffffffffu, ks, group_page), vg = __shfl_sync(0xffffffffu, vs, group_page);
+      if (lane < 4) {
+        const float lv = __log2f(vg);
+        b.scale[j & 3][lane] = make_float4(kg, lv, exp2_approx(-lv), 0.f);
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&b.scale_full[j & 3]);
+      mbar_arrive(&b.k_full[st]);
+      if (!__all_sync(0xffffffffu, mbar_wait(&b.v_empty[st], free_parity))) {
+        report_wait(a.err, kErrTimeoutProducer, 52, a.total_rows, it.splits);
+        (void)mbar_wait(&b.k_full[st], (j >> 1) & 1u);  // its K copies land first
+        break;
+      }
+      if (live) load(&tm_v, &b.v_full[st], smem + kOffV + st * kTile);
+      mbar_arrive(&b.v_full[st]);
+      __syncwarp();
+    }
+    for (int j = max(0, issued - 2); j < issued; ++j)  // every copy landed before leaving
+      if (!mbar_wait(&b.k_full[j & 1], (j >> 1) & 1u) || !mbar_wait(&b.v_full[j & 1], (j >> 1) & 1u)) break;
+  } else if (warp == 1) {
+    if (lane == 0) {
+      // ---------------- MMA issuer ----------------
+      int site = 0;
+      if (!mbar_wait(&b.q_ready, 0)) site = 53;
+      const uint64_t qh = umma_desc_sw128(smem + kOffQ), ql = umma_desc_sw128(smem + kOffQ + kQ);
+      for (int j = 0; j <= n_tiles && site == 0; ++j) {
+        if (j < n_tiles) {  // S_j = (Qh + Ql) K_j^T, into the buffer that P_{j-2} has left
+          const int st = j & 1;
+          if (!mbar_wait(&b.k_full[st], (j >> 1) & 1u)) {
+            site = 54;
+            break;
+          }
+          if (j >= 2 && !mbar_wait(&b.pv_done[st], ((j - 2) >> 1) & 1u)) {
+            site = 55;
+            break;
+          }
+          tc_fence_after_sync();
+          const uint64_t kd = umma_desc_sw128(smem + kOffK + st * kTile);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            mma_f8(tmem + kTmemS + st * kKeys, qh + 2 * k, kd + 2 * k, kIdescS, k > 0 ? 1u : 0u);
+            mma_f8(tmem + kTmemS + st * kKeys, ql + 2 * k, kd + 2 * k, kIdescS, 1u);
+          }
+          tc_commit(&b.s_full[st]);
+          tc_commit(&b.k_empty[st]);
+        }
+        if (j >= 1) {  // O += P_i V_i, i = j - 1
+          const int i = j - 1, buf = i & 1;
+          if (!mbar_wait(&b.w_full[buf], (i >> 1) & 1u)) {
+            site = 56;
+            break;
+          }
+          if (!mbar_wait(&b.p_full[buf], (i >> 1) & 1u)) {
+            site = 57;
+            break;
+          }
+          tc_fence_after_sync();
+#pragma unroll
+          for (int k = 0; k < 4; ++k)  // 16 keys a step: 8 columns of P, two 8-row groups of V
+            mma_f16_ta(tmem + kTmemO, tmem + kTmemS + buf * kKeys + 8 * k,
+                       umma_desc_sw128_mn(smem + kOffV16 + buf * kV16 + k * 2048, kV16 / 2, 1024), kIdescO,
+                       (i > 0 || k > 0) ? 1u : 0u);
+          tc_commit(&b.pv_done[buf]);
+          if (i == n_tiles - 1) tc_commit(&b.o_final);
+        }
+      }
+      if (site != 0) report_wait(a.err, kErrTimeoutMma, site, a.total_rows, it.splits);
+    }
+  } else if (warp >= 8) {
+    set_registers<kRegsWiden, false>();
+    // ---------------- V in f16: a key a lane, half a row a thread ----------------
+    const int half = warp & 1, k = 32 * ((warp - 8) >> 1) + lane;  // key of the tile
+    bool ok = true;
+    for (int j = 0; j < n_tiles && ok; ++j) {
+      const int st = j & 1;
+      ok = __all_sync(0xffffffffu, mbar_wait(&b.v_full[st], (j >> 1) & 1u));
+      if (!ok) break;
+      const uint8_t* src = smem + kOffV + st * kTile + k * kHd;
+      // rows past the range hold anything: their weight is 0, their values must be
+      const bool dead = it.key0 + j * kKeys + k >= it.key1;
+      uint4 u[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        u[c] = *reinterpret_cast<const uint4*>(src + (((4 * half + c) ^ (k & 7)) << 4));
+        if (dead) u[c] = make_uint4(0u, 0u, 0u, 0u);
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&b.v_empty[st]);
+      if (j >= 2) {  // P_{j-2} V_{j-2} has left the buffer
+        ok = __all_sync(0xffffffffu, mbar_wait(&b.pv_done[st], ((j - 2) >> 1) & 1u));
+        if (!ok) break;
+      }
+      uint8_t* dst = smem + kOffV16 + st * kV16 + half * (kV16 / 2) + k * 128;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const uint32_t e[4] = {u[c].x, u[c].y, u[c].z, u[c].w};
+        uint32_t f[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          f[2 * i] = f16x2_from_e4m3x2(static_cast<uint16_t>(e[i]));
+          f[2 * i + 1] = f16x2_from_e4m3x2(static_cast<uint16_t>(e[i] >> 16));
+        }
+        *reinterpret_cast<uint4*>(dst + (((2 * c) ^ (k & 7)) << 4)) = make_uint4(f[0], f[1], f[2], f[3]);
+        *reinterpret_cast<uint4*>(dst + (((2 * c + 1) ^ (k & 7)) << 4)) = make_uint4(f[4], f[5], f[6], f[7]);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&b.w_full[st]);
+    }
+    if (!ok && lane == 0) report_wait(a.err, kErrTimeoutEpilogue, 58, a.total_rows, it.splits);
+  } else if (warp >= 4) {
+    set_registers<kRegsSoftmax, true>();
+    // ---------------- softmax and output: a row a thread ----------------
+    const int q4 = warp & 3, tid = q4 * 32 + lane;
+    const uint32_t lane_base = static_cast<uint32_t>(q4 * 32) << 16;
+    const bool valid = tid < it.rows;
+    const int t = (it.row0 + (valid ? tid : 0)) / G, head = it.head * G + (it.row0 + (valid ? tid : 0)) % G;
+    const int lim = valid ? min(it.key1, paged_key_limit(it.len, it.start + t, a.causal_block)) : it.key0;
+    float unscale;
+    {  // the query row -> Qh, Ql with the 128-byte swizzle (zeros for padding rows)
+      const uint4* src = reinterpret_cast<const uint4*>(static_cast<const bf16*>(a.q) + static_cast<size_t>(it.tok0 + t) * a.ldq +
+                                                        static_cast<size_t>(head) * kHd);
+      uint4 v[16];
+#pragma unroll
+      for (int c = 0; c < 16; ++c) v[c] = valid ? src[c] : make_uint4(0u, 0u, 0u, 0u);
+      float m = 0.f;
+#pragma unroll
+      for (int c = 0; c < 16; ++c) {
+        const uint32_t w[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          m = fmaxf(m, fmaxf(fabsf(__uint_as_float(w[i] << 16)), fabsf(__uint_as_float(w[i] & 0xFFFF0000u))));
+      }
+      // exponent of m, kept where both the scale and its inverse are normal floats
+      const int e = min(max(static_cast<int>(__float_as_uint(m) >> 23) - 127, -110), 110);
+      const float up = m > 0.f ? __uint_as_float(static_cast<uint32_t>(127 + 7 - e) << 23) : 1.f;
+      unscale = a.scale * kLog2e / up;
+      uint8_t* dst = smem + kOffQ + tid * kHd;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint4& u = v[2 * c + (i >> 1)];
+          const uint32_t w0 = i & 1 ? u.z : u.x, w1 = i & 1 ? u.w : u.y;
+          const float x0 = __uint_as_float(w0 << 16) * up, x1 = __uint_as_float(w0 & 0xFFFF0000u) * up;
+          const float x2 = __uint_as_float(w1 << 16) * up, x3 = __uint_as_float(w1 & 0xFFFF0000u) * up;
+          const uint16_t c0 = e4m3x2_from_f32(x0, x1), c1 = e4m3x2_from_f32(x2, x3);
+          const float2 r0 = f32x2_from_e4m3x2(c0), r1 = f32x2_from_e4m3x2(c1);
+          hi[i] = c0 | static_cast<uint32_t>(c1) << 16;
+          lo[i] = e4m3x2_from_f32(x0 - r0.x, x1 - r0.y) | static_cast<uint32_t>(e4m3x2_from_f32(x2 - r1.x, x3 - r1.y)) << 16;
+        }
+        *reinterpret_cast<uint4*>(dst + ((c ^ (tid & 7)) << 4)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        *reinterpret_cast<uint4*>(dst + kQ + ((c ^ (tid & 7)) << 4)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      }
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&b.q_ready);
+
+    float base = 0.f, l = 0.f;
+    bool ok = true, seated = false;  // seated: the base has been set (the row has attended a key)
+    for (int j = 0; j < n_tiles; ++j) {
+      const int sb = j & 1, key0 = it.key0 + j * kKeys;
+      ok = __all_sync(0xffffffffu, mbar_wait(&b.scale_full[j & 3], (j >> 2) & 1u) && mbar_wait(&b.s_full[sb], (j >> 1) & 1u));
+      if (!ok) break;
+      tc_fence_after_sync();
+      const uint32_t s_at = tmem + lane_base + kTmemS + sb * kKeys;
+      float x[kKeys];
+      {
+        uint32_t v0[32], v1[32];
+        tmem_ld_32x32b_x32(s_at, v0);
+        tmem_ld_32x32b_x32(s_at + 32, v1);
+        tmem_ld_wait();
+        after_wait(v0);
+        after_wait(v1);
+#pragma unroll
+        for (int c = 0; c < 32; ++c) x[c] = __uint_as_float(v0[c]), x[32 + c] = __uint_as_float(v1[c]);
+      }
+      float inv_vs[4];
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const float4 sc = b.scale[j & 3][g];
+        const float m = unscale * sc.x, c = sc.y - base;
+        inv_vs[g] = sc.z;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[16 * g + i] = fmaf(x[16 * g + i], m, c);
+      }
+      if (__any_sync(0xffffffffu, key0 + kKeys > lim)) {  // (also what keys past the range gave)
+#pragma unroll
+        for (int c = 0; c < kKeys; ++c)
+          if (key0 + c >= lim) x[c] = -INFINITY;
+      }
+      float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int c = 0; c < kKeys; ++c) top[c & 3] = fmaxf(top[c & 3], x[c]);
+      const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+      const bool move = mx < INFINITY && (mx > kTrip || (!seated && mx > -INFINITY));
+      if (__any_sync(0xffffffffu, move)) {
+        const float d = move ? kSeat - mx : 0.f, f = exp2_approx(d);  // new weights are 2^d times the old
+        if (__any_sync(0xffffffffu, move && seated)) {  // O holds earlier tiles: their last product has to land first
+          ok = __all_sync(0xffffffffu, mbar_wait(&b.pv_done[(j - 1) & 1], ((j - 1) >> 1) & 1u));
+          if (!ok) break;
+          tc_fence_after_sync();
+#pragma unroll 1
+          for (int c0 = 0; c0 < kHd; c0 += 32) {
+            uint32_t v[32];
+            tmem_ld_32x32b_x32(tmem + lane_base + kTmemO + c0, v);
+            tmem_ld_wait();
+            after_wait(v);
+#pragma unroll
+            for (int c = 0; c < 32; ++c) v[c] = __float_as_uint(__uint_as_float(v[c]) * (seated ? f : 1.f));
+            tmem_st_32x32b_x32(tmem + lane_base + kTmemO + c0, v);
+          }
+          tmem_st_wait();
+        }
+        base -= d;
+        l *= seated ? f : 1.f;
+        seated |= move;
+#pragma unroll
+        for (int c = 0; c < kKeys; ++c) x[c] += d;
+      }
+      uint32_t w[32];
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        float p0 = 0.f, p1 = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+          const float e0 = exp2_approx(x[16 * g + i]), e1 = exp2_approx(x[16 * g + i + 1]);
+          p0 += e0;
+          p1 += e1;
+          w[8 * g + i / 2] = pack_f16x2(e0, e1);
+        }
+        l = fmaf(p0 + p1, inv_vs[g], l);
+      }
+      tmem_st_32x32b_x32(s_at, w);  // P_j over S_j
+      tmem_st_wait();
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&b.p_full[sb]);
+    }
+    ok = __all_sync(0xffffffffu, ok && mbar_wait(&b.o_final, 0));
+    if (!ok && lane == 0) report_wait(a.err, kErrTimeoutEpilogue, 59, a.total_rows, it.splits);
+    tc_fence_after_sync();
+    // a split tile leaves its partial: [128][128], then [128] (base, sum)
+    const float inv = it.splits > 1 ? 1.f : l != 0.f ? 1.f / l : 0.f;
+    uint4* out = reinterpret_cast<uint4*>(static_cast<bf16*>(a.out) + (static_cast<size_t>(it.tok0 + t) * a.hq + head) * kHd);
+    float4* part = a.part + it.part;
+#pragma unroll 1
+    for (int c0 = 0; c0 < kHd; c0 += 32) {
+      uint32_t v[32];
+      tmem_ld_32x32b_x32(tmem + lane_base + kTmemO + c0, v);
+      tmem_ld_wait();
+      after_wait(v);
+      if (!valid) continue;
+      auto at = [&](int c) { return __uint_as_float(v[c]) * inv; };
+      if (it.splits == 1) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          out[c0 / 8 + c] = make_uint4(pack_bf16x2(at(8 * c), at(8 * c + 1)), pack_bf16x2(at(8 * c + 2), at(8 * c + 3)),
+                                       pack_bf16x2(at(8 * c + 4), at(8 * c + 5)), pack_bf16x2(at(8 * c + 6), at(8 * c + 7)));
+      } else {
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+          part[tid * (kHd / 4) + c0 / 4 + c] = make_float4(at(4 * c), at(4 * c + 1), at(4 * c + 2), at(4 * c + 3));
+      }
+    }
+    if (it.splits > 1) {
+      if (valid) reinterpret_cast<float2*>(part + kRows * (kHd / 4))[tid] = make_float2(base, l);
+      __threadfence();
+    }
+    tc_fence_before_sync();
+  }
+  __syncwarp();
+  tc_fence_before_sync();
+  __syncthreads();
+  // Back to the launch's split.  Only here, past the barrier: a warp without a role that took its registers
+  // back any earlier would leave the softmax waiting for them.
+  if (warp >= 4 && warp < 8) set_registers<kRegsLaunch, false>();
+  else set_registers<kRegsLaunch, true>();
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem, kTmemCols);
+  }
+  if (it.splits == 1) return;
+
+  // the tile's last item adds the partials, all threads: a row's weights 2^(base - max) / sum, then its columns
+  if (threadIdx.x == 0) b.last = atomicAdd(&a.arrived[it.tile], 1u) == static_cast<unsigned>(it.splits - 1);
+  __syncthreads();
+  if (!b.last) return;
+  __threadfence();
+  constexpr int kPart = kRows * kHd + 4 * kRows;  // floats
+  const float* first = reinterpret_cast<const float*>(a.part + it.part) - static_cast<size_t>(it.split) * kPart;
+  float* weight = reinterpret_cast<float*>(smem);  // [kMaxPagedSplits][128], over the queries
+  if (threadIdx.x < it.rows) {
+    const int n = threadIdx.x;
+    float m = -INFINITY;
+#pragma unroll 8
+    for (int s = 0; s < it.splits; ++s) {
+      const float2 bs = __ldcg(reinterpret_cast<const float2*>(first + s * kPart + kRows * kHd) + n);
+      weight[s * kRows + n] = bs.x;
+      if (bs.y != 0.f) m = fmaxf(m, bs.x);
+    }
+    float l = 0.f;
+#pragma unroll 8
+    for (int s = 0; s < it.splits; ++s) {
+      const float2 bs = __ldcg(reinterpret_cast<const float2*>(first + s * kPart + kRows * kHd) + n);
+      const float f = bs.y != 0.f ? exp2f(bs.x - m) : 0.f;
+      weight[s * kRows + n] = f;
+      l += f * bs.y;
+    }
+    const float inv = l != 0.f ? 1.f / l : 0.f;
+    for (int s = 0; s < it.splits; ++s) weight[s * kRows + n] *= inv;
+  }
+  __syncthreads();
+#pragma unroll 2
+  for (int i = threadIdx.x; i < it.rows * (kHd / 4); i += kThreads) {
+    const int n = i >> 5, c4 = i & 31, row = it.row0 + n;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int s = 0; s < it.splits; ++s) {
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(first + s * kPart + n * kHd) + c4);
+      const float f = weight[s * kRows + n];
+      acc.x += f * v.x, acc.y += f * v.y, acc.z += f * v.z, acc.w += f * v.w;
+    }
+    bf16* dst = static_cast<bf16*>(a.out) + (static_cast<size_t>(it.tok0 + row / G) * a.hq + it.head * G + row % G) * kHd + 4 * c4;
+    *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(acc.x, acc.y), pack_bf16x2(acc.z, acc.w));
+  }
+  if (threadIdx.x == 0) a.arrived[it.tile] = 0;  // ready for the next call
+}
+
+// The register split only ever asks for what the launch brought: checked here, not by waiting for more.
+int init_paged_attention_wide_attributes() {
+  cudaFuncAttributes f;
+  cudaError_t e = cudaFuncGetAttributes(&f, paged_attn_wide_kernel);
+  if (e == cudaSuccess && f.numRegs < kRegsLaunch) e = cudaErrorInvalidKernelImage;
+  return e != cudaSuccess ? e : cudaFuncSetAttribute(paged_attn_wide_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
+}
+
+int launch_paged_attention_wide(const PagedAttnArgs& a, int n_items, const CUtensorMap& k, const CUtensorMap& v,
+                                cudaStream_t s) {
+  return launch_k(paged_attn_wide_kernel, dim3(n_items), dim3(kThreads), kBytes, s, a, k, v);
+}
+
+}  // namespace fdllm
