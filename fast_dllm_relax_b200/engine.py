@@ -27,6 +27,9 @@ from .paged import PagedCache, PagedPlan
 _DT = {"float32": (torch.float32, 0), "bfloat16": (torch.bfloat16, 1)}
 
 
+_LOGITS_DT = {torch.float32: 0, torch.bfloat16: 1}
+
+
 def _ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
@@ -45,6 +48,9 @@ class Engine:
             device = torch.cuda.current_device()
         self.device = torch.device("cuda", torch.device(device).index if isinstance(device, torch.device) else int(device))
         self.lib = _lib.load()
+        self._q_cols = cfg.num_attention_heads * cfg.head_dim
+        self._kv_cols = cfg.num_key_value_heads * cfg.head_dim
+        self._esz = 2 if dtype == "bfloat16" else 4
         self._cache_ok: dict = {}  # id(k) -> (ref(k), ref(v), shape): caches validated before
         c = _lib.FdllmConfig(cfg.vocab_size, cfg.hidden_size, cfg.intermediate_size, cfg.num_hidden_layers,
                              cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim, cfg.rms_norm_eps,
@@ -285,17 +291,21 @@ class Engine:
         targets [rows] ids or None.  Returns (logprob [rows] or None, entropy [rows] in nats, top_ids
         int32 [rows, top], top_logprobs [rows, top]): the `top` (up to 32) largest in order, ties to
         the lowest id."""
-        codes = {torch.float32: 0, torch.bfloat16: 1}
         x = logits[0] if logits.dim() == 3 and logits.shape[0] == 1 else logits
-        if x.dim() != 2 or x.dtype not in codes or x.device != self.device:
+        code = _LOGITS_DT.get(x.dtype)
+        if x.dim() != 2 or code is None or x.device != self.device:
             raise ValueError(f"logprobs: expected fp32 or bf16 logits [rows, vocab] on {self.device}, got "
                              f"{x.dtype} {tuple(x.shape)} on {x.device}")
         n, vocab = x.shape
-        if (vocab > 1 and x.stride(1) != 1) or (n > 1 and x.stride(0) < vocab):
+        ld, one = x.stride()
+        if (vocab > 1 and one != 1) or (n > 1 and ld < vocab):
             x = x.contiguous()
+            ld = vocab
         tg = lp = None
         if targets is not None:
-            tg = targets.to(self.device, torch.int32).contiguous().reshape(-1)
+            tg = targets
+            if tg.dtype is not torch.int32 or tg.device != self.device or tg.dim() != 1 or not tg.is_contiguous():
+                tg = tg.to(self.device, torch.int32).contiguous().reshape(-1)
             if tg.numel() != n:
                 raise ValueError("logprobs: one target per row")
             lp = torch.empty(n, dtype=torch.float32, device=self.device)
@@ -303,10 +313,9 @@ class Engine:
         top = int(top)
         ids = torch.empty((n, max(top, 0)), dtype=torch.int32, device=self.device)
         tlp = torch.empty((n, max(top, 0)), dtype=torch.float32, device=self.device)
-        _lib.check(self.lib.fdllm_logprobs(self._h, x.data_ptr(), codes[x.dtype], n, vocab,
-                                           int(x.stride(0)) if n > 1 else vocab, _ptr(tg), top, _ptr(lp),
-                                           ent.data_ptr(), ids.data_ptr() if top > 0 else None,
-                                           tlp.data_ptr() if top > 0 else None, self._stream()))
+        _lib.check(self.lib.fdllm_logprobs(self._h, x.data_ptr(), code, n, vocab, ld if n > 1 else vocab, _ptr(tg), top,
+                                           _ptr(lp), ent.data_ptr(), ids.data_ptr() if top > 0 else None,
+                                           tlp.data_ptr() if top > 0 else None, self._raw_stream()))
         return lp, ent, ids, tlp
 
     # ---- paged 8-bit cache --------------------------------------------------------------------
@@ -344,25 +353,28 @@ class Engine:
         head_dim] before RoPE; views of a packed qkv tensor are taken as they are.  table: int32
         [n, columns] page ids.  rope: fp32 (cos, sin) tables [positions, head_dim / 2], else the
         engine's.  Returns the rotated queries."""
-        c = self.cfg
-        pc = self._paged(cache, plan, table, "paged_append")
-        cols = (c.num_attention_heads * c.head_dim, c.num_key_value_heads * c.head_dim)
-        q = None if q is None else self._token_rows(q, plan, cols[0], "paged_append: q")
-        k, v = (self._token_rows(t, plan, cols[1], f"paged_append: {s}") for t, s in ((k, "k"), (v, "v")))
+        self._paged(cache, plan, table, "paged_append")
+        rows, q_cols, kv_cols = plan.total_rows, self._q_cols, self._kv_cols
+        k = self._token_rows(k, rows, kv_cols, "paged_append: k")
+        v = self._token_rows(v, rows, kv_cols, "paged_append: v")
+        out = None
+        if q is not None:
+            q = self._token_rows(q, rows, q_cols, "paged_append: q")
+            out = torch.empty((rows, q_cols), dtype=self.dtype, device=self.device)
         cos = sin = None
+        positions = 0
         if rope is not None:
             cos, sin = rope
+            half = self.cfg.head_dim // 2
             for t in (cos, sin):
                 if t.device != self.device or t.dtype != torch.float32 or t.dim() != 2 or not t.is_contiguous() \
-                        or t.shape[1] != c.head_dim // 2 or t.shape != cos.shape:
-                    raise ValueError(f"paged_append: rope tables must be contiguous fp32 [positions, {c.head_dim // 2}] "
-                                     f"on {self.device}")
-        out = None if q is None else torch.empty((plan.total_rows, cols[0]), dtype=self.dtype, device=self.device)
+                        or t.shape[1] != half or t.shape != cos.shape:
+                    raise ValueError(f"paged_append: rope tables must be contiguous fp32 [positions, {half}] on {self.device}")
+            positions = cos.shape[0]
         _lib.check(self.lib.fdllm_paged_append(
-            self._h, ctypes.byref(pc), int(layer), ctypes.byref(plan.desc), plan.words.data_ptr(), table.data_ptr(),
-            int(table.shape[1]), _ptr(q), 0 if q is None else int(q.stride(0)), k.data_ptr(), int(k.stride(0)),
-            v.data_ptr(), int(v.stride(0)), _ptr(cos), _ptr(sin), 0 if cos is None else int(cos.shape[0]), _ptr(out),
-            self._stream()))
+            self._h, cache.ref, layer, plan.ref, plan.words_ptr, table.data_ptr(), table.shape[1], _ptr(q),
+            0 if q is None else q.stride(0), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), _ptr(cos), _ptr(sin),
+            positions, _ptr(out), self._raw_stream()))
         return out
 
     def paged_attention(self, cache: PagedCache, layer: int, plan: PagedPlan, table: torch.Tensor, q: torch.Tensor,
@@ -370,15 +382,13 @@ class Engine:
         """Attention of the plan's token rows over `layer` of the cache (fdllm_paged_attention): q
         [total_rows, heads * head_dim], rotated -> [total_rows, heads * head_dim].  scale defaults to
         head_dim ** -0.5."""
-        c = self.cfg
-        pc = self._paged(cache, plan, table, "paged_attention")
-        cols = c.num_attention_heads * c.head_dim
-        q = self._token_rows(q, plan, cols, "paged_attention: q")
-        out = torch.empty((plan.total_rows, cols), dtype=self.dtype, device=self.device)
+        self._paged(cache, plan, table, "paged_attention")
+        rows = plan.total_rows
+        q = self._token_rows(q, rows, self._q_cols, "paged_attention: q")
+        out = torch.empty((rows, self._q_cols), dtype=self.dtype, device=self.device)
         _lib.check(self.lib.fdllm_paged_attention(
-            self._h, ctypes.byref(pc), int(layer), ctypes.byref(plan.desc), plan.words.data_ptr(), table.data_ptr(),
-            int(table.shape[1]), q.data_ptr(), int(q.stride(0)), float(c.head_dim ** -0.5 if scale is None else scale),
-            out.data_ptr(), self._stream()))
+            self._h, cache.ref, layer, plan.ref, plan.words_ptr, table.data_ptr(), table.shape[1], q.data_ptr(),
+            q.stride(0), self.cfg.head_dim ** -0.5 if scale is None else scale, out.data_ptr(), self._raw_stream()))
         return out
 
     def generate(self, prompt_ids: Sequence[int], *, max_new_tokens: int, block_size: int = 32,
@@ -453,31 +463,33 @@ class Engine:
         return int(self.lib.fdllm_workspace_bytes(self._h))
 
     # ---- argument normalisation --------------------------------------------------------------
-    def _paged(self, cache: PagedCache, plan: PagedPlan, table: torch.Tensor, name: str):
+    def _paged(self, cache: PagedCache, plan: PagedPlan, table: torch.Tensor, name: str) -> None:
         c = self.cfg
-        if cache.k.device != self.device or cache.k.shape[2] != c.num_key_value_heads or cache.k.shape[4] != c.head_dim:
+        if cache.heads != (c.num_key_value_heads, c.head_dim) or cache.device != self.device:
             raise ValueError(f"{name}: cache must be [layers, pages, {c.num_key_value_heads}, page_size, {c.head_dim}] on "
-                             f"{self.device}, got {tuple(cache.k.shape)} on {cache.k.device}")
-        if table.dim() != 2 or table.dtype != torch.int32 or table.device != self.device or not table.is_contiguous() \
-                or table.shape[0] != plan.desc.n:
-            raise ValueError(f"{name}: table must be a contiguous int32 [{plan.desc.n}, columns] tensor on {self.device}")
-        if plan.words.device != self.device:
-            raise ValueError(f"{name}: the plan is on {plan.words.device}")
-        return _lib.FdllmPagedCache(cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(),
-                                    cache.v_scale.data_ptr(), cache.layers, cache.pages, cache.page_size)
+                             f"{self.device}, got {tuple(cache.k.shape)} on {cache.device}")
+        if table.dim() != 2 or table.shape[0] != plan.n or table.dtype is not torch.int32 \
+                or table.device != self.device or not table.is_contiguous():
+            raise ValueError(f"{name}: table must be a contiguous int32 [{plan.n}, columns] tensor on {self.device}")
+        if plan.device != self.device:
+            raise ValueError(f"{name}: the plan is on {plan.device}")
 
-    def _token_rows(self, t: torch.Tensor, plan: PagedPlan, cols: int, name: str) -> torch.Tensor:
-        """[total_rows, cols] in the engine's dtype with 16-byte aligned rows: strided views pass as they
-        are, others are copied."""
-        if t.device != self.device or t.dtype != self.dtype or t.dim() < 2 or t.shape[0] != plan.total_rows \
-                or t[:1].numel() != (cols if plan.total_rows else 0):
-            raise ValueError(f"{name}: expected {self.dtype} [{plan.total_rows}, {cols}] on {self.device}, got "
-                             f"{t.dtype} {tuple(t.shape)} on {t.device}")
-        t = t.reshape(plan.total_rows, cols)
-        unit = 16 // t.element_size()
-        if t.stride(1) != 1 or t.stride(0) < cols or t.stride(0) % unit or t.data_ptr() % 16:
+    def _token_rows(self, t: torch.Tensor, rows: int, cols: int, name: str) -> torch.Tensor:
+        """[rows, cols] in the engine's dtype with 16-byte aligned rows: strided views pass as they are,
+        others are copied."""
+        if t.dim() != 2:
+            t = t.reshape(rows, cols) if t.dim() > 2 and t.shape[0] == rows and t[:1].numel() == cols else t
+        if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != cols or t.dtype is not self.dtype or t.device != self.device:
+            raise ValueError(f"{name}: expected {self.dtype} [{rows}, {cols}] on {self.device}, got {t.dtype} "
+                             f"{tuple(t.shape)} on {t.device}")
+        ld, one = t.stride()
+        if one != 1 or ld < cols or (ld * self._esz | t.data_ptr()) & 15:
             t = t.contiguous() if not t.is_contiguous() else t.clone()
         return t
+
+    def _raw_stream(self) -> int:
+        """torch's current stream on the engine's device, without building a Stream object."""
+        return torch._C._cuda_getCurrentRawStream(self.device.index)
 
     def _bias(self, bias: torch.Tensor | None, T: int) -> torch.Tensor | None:
         if bias is None:

@@ -9,17 +9,21 @@
 
 from __future__ import annotations
 
+import ctypes
 import dataclasses
 
 import torch
 
+from . import _lib
+
 PAGE_SIZES = (16, 32, 64, 128)
 
 
-@dataclasses.dataclass
+@dataclasses.dataclass(frozen=True, eq=False)
 class PagedCache:
     """A pool of pages: float8 e4m3 codes [layers, pages, kv_heads, page_size, head_dim] of the keys
-    and of the values, and fp32 scales [layers, pages, kv_heads]; a cached value is code * scale."""
+    and of the values, and fp32 scales [layers, pages, kv_heads]; a cached value is code * scale.
+    Immutable (its tensors' contents are not), so that it is checked once, not in every layer's call."""
 
     k: torch.Tensor
     v: torch.Tensor
@@ -39,6 +43,12 @@ class PagedCache:
                 raise ValueError("paged cache: scales must be contiguous float32 [layers, pages, kv_heads]")
         if len({t.device for t in (self.k, self.v, self.k_scale, self.v_scale)}) != 1:
             raise ValueError("paged cache: tensors on different devices")
+        desc = _lib.FdllmPagedCache(self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(),
+                                    self.v_scale.data_ptr(), self.layers, self.pages, self.page_size)
+        object.__setattr__(self, "device", self.k.device)
+        object.__setattr__(self, "heads", (int(self.k.shape[2]), int(self.k.shape[4])))  # KV heads, head dim
+        object.__setattr__(self, "_desc", desc)
+        object.__setattr__(self, "ref", ctypes.byref(desc))
 
     @property
     def layers(self) -> int:
@@ -61,11 +71,9 @@ class PagedPlan:
         self.desc = desc
         self.words = words
         self._staging = staging  # pinned source of the upload, alive as long as the plan
-
-    @property
-    def total_rows(self) -> int:
-        return int(self.desc.total_rows)
-
-    @property
-    def table_cols(self) -> int:
-        return int(self.desc.table_cols)
+        self.ref = ctypes.byref(desc)
+        self.words_ptr = words.data_ptr()
+        self.device = words.device
+        self.n = int(desc.n)
+        self.total_rows = int(desc.total_rows)
+        self.table_cols = int(desc.table_cols)  # columns a page table needs
