@@ -187,7 +187,7 @@ int fdllm_paged_plan_batch(fdllm_handle* h, const int32_t* rows, const int32_t* 
     if (!page_size_ok(page_size)) return fail(FDLLM_ERR_INVALID, "page size must be 16, 32, 64 or 128");
     if (causal_block < 0) return fail(FDLLM_ERR_INVALID, "causal_block must not be negative");
     std::vector<PagedReq> reqs(n);
-    std::vector<PagedPageUnit> units;
+    std::vector<PagedPageUnit> units, q_units;
     long long total = 0, max_len = 0, max_pos = 0;
     for (int i = 0; i < n; ++i) {
       const long long r = rows[i], s = start[i], lv = live != nullptr ? live[i] : start[i];
@@ -203,6 +203,7 @@ int fdllm_paged_plan_batch(fdllm_handle* h, const int32_t* rows, const int32_t* 
       if (r > 0) max_pos = std::max(max_pos, s + r);
       for (long long p = s / page_size; r > 0 && p <= (s + r - 1) / page_size; ++p)
         units.push_back(PagedPageUnit{i, static_cast<int>(p)});
+      for (long long t = 0; t < r; t += kPagedQTokens) q_units.push_back(PagedPageUnit{i, static_cast<int>(t)});
     }
     fdllm_paged_plan out{};
     out.n = n;
@@ -215,6 +216,9 @@ int fdllm_paged_plan_batch(fdllm_handle* h, const int32_t* rows, const int32_t* 
     out.priv[kPagedPageUnits] = static_cast<int>(units.size());
     out.priv[kPagedPageOff] = at;
     at += 2 * static_cast<int>(units.size());
+    out.priv[kPagedQUnits] = static_cast<int>(q_units.size());
+    out.priv[kPagedQOff] = at;
+    at += 2 * static_cast<int>(q_units.size());
     at = (at + 3) & ~3;  // items are read in 16-byte words
     ItemPlan ip;
     if (h->dtype == FDLLM_BFLOAT16) FDLLM_TRY(plan_items(h, reqs, causal_block, &ip));
@@ -235,6 +239,8 @@ int fdllm_paged_plan_batch(fdllm_handle* h, const int32_t* rows, const int32_t* 
     if (n > 0) std::memcpy(words, reqs.data(), reqs.size() * sizeof(PagedReq));
     if (!units.empty())
       std::memcpy(words + out.priv[kPagedPageOff], units.data(), units.size() * sizeof(PagedPageUnit));
+    if (!q_units.empty())
+      std::memcpy(words + out.priv[kPagedQOff], q_units.data(), q_units.size() * sizeof(PagedPageUnit));
     for (int c = 0; c < kPagedClasses; ++c)
       if (!ip.items[c].empty())
         std::memcpy(words + out.priv[kPagedItemOff + c], ip.items[c].data(), ip.items[c].size() * sizeof(PagedItem));
@@ -270,6 +276,8 @@ int fdllm_paged_append(fdllm_handle* h, const fdllm_paged_cache* cache, int laye
     a.reqs = reinterpret_cast<const PagedReq*>(plan_words);
     a.units = reinterpret_cast<const PagedPageUnit*>(plan_words + plan->priv[kPagedPageOff]);
     a.n_units = plan->priv[kPagedPageUnits];
+    a.q_units = reinterpret_cast<const PagedPageUnit*>(plan_words + plan->priv[kPagedQOff]);
+    a.n_q_units = plan->priv[kPagedQUnits];
     a.n = plan->n;
     a.total_rows = plan->total_rows;
     a.table = table;

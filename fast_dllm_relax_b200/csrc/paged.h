@@ -23,10 +23,12 @@ struct PagedReq {
 };
 static_assert(sizeof(PagedReq) == 4 * kPagedReqWords, "plan request layout");
 
-// One page that an append writes: words[page_off + 2 * u].
+// A CTA's share of an append, two words: one page that it writes, or up to kPagedQTokens token rows whose
+// queries it rotates.
+constexpr int kPagedQTokens = 16;
 struct PagedPageUnit {
   int req;
-  int slot;  // page number within the request
+  int slot;  // page number within the request / first token row within it
 };
 
 constexpr int kMaxPagedSplits = 32;  // key shares of a tile (a lane each in the join)
@@ -59,12 +61,15 @@ enum PagedPriv : int {
   kPagedParts = 3,      // workspace for partials, in 16-byte units
   kPagedItems = 4,      // [kPagedClasses] numbers of items
   kPagedItemOff = kPagedItems + kPagedClasses,  // [kPagedClasses] word offsets of the items
+  kPagedQUnits = kPagedItemOff + kPagedClasses,  // number of query units
+  kPagedQOff,           // word offset of the query units
+  kPagedPrivEnd,
 };
 
 struct PagedAppendArgs {
   const PagedReq* reqs;
-  const PagedPageUnit* units;
-  int n_units, n, total_rows;
+  const PagedPageUnit *units, *q_units;
+  int n_units, n_q_units, n, total_rows;
   const int* table;
   int table_ld;
   uint8_t *k, *v;          // this layer's codes [pages, hkv, page_size, hd]
@@ -148,6 +153,8 @@ __device__ __forceinline__ float2 f32x2_from_e4m3x2(uint16_t c) {
   const uint32_t h = f16x2_from_e4m3x2(c);
   return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
+
+static_assert(kPagedPrivEnd <= 17, "fdllm_paged_plan::priv");
 
 // The request that owns token row `tok`: the last one with tok0 <= tok (empty requests share the
 // tok0 of the next one, so the last is the owner).

@@ -9,6 +9,15 @@
 //
 // A power of two makes both divisions exact, so a value is rounded once, and a kept code only loses
 // bits where it becomes subnormal.
+//
+// Bound: HBM (every input read once, every output written once).  One launch, two kinds of CTAs:
+//   - a page, KV head and K or V: a thread holds up to two 8-column chunk pairs (K) or four chunks (V) of the
+//     page's new rows in registers, so the values are read and rotated once, reduced to the page's maximum across
+//     the CTA, and coded from the registers;
+//   - up to 16 token rows of one request for the queries: a thread holds its position's 8 cosines and sines and
+//     applies them to every head of its share.
+#include <algorithm>
+
 #include "paged.h"
 
 namespace fdllm {
@@ -32,39 +41,101 @@ __device__ __forceinline__ float finite_abs(float x) {
   return a < INFINITY ? a : 0.f;  // NaN and infinities do not move the scale
 }
 
-template <typename TT>
-__device__ __forceinline__ float table_at(const void* t, size_t i) { return to_f<TT>(static_cast<const TT*>(t)[i]); }
-
-// Value d of the rotated (or plain, V) row.
-template <typename T, typename TT>
-__device__ __forceinline__ float new_value(const T* row, int d, int hd, bool rotate, const PagedAppendArgs& a, int pos) {
-  const float x = to_f<T>(row[d]);
-  if (!rotate) return x;
-  const int half = hd >> 1, i = d < half ? d : d - half;
-  const size_t at = static_cast<size_t>(pos) * half + i;
-  const float c = table_at<TT>(a.cos, at), s = table_at<TT>(a.sin, at);
-  const float y = to_f<T>(row[d < half ? d + half : d - half]);
-  return d < half ? x * c - y * s : x * c + y * s;
+// Eight consecutive values, 16-byte aligned (bf16) or 32 bytes in two loads (fp32).
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float (&x)[8]);
+template <>
+__device__ __forceinline__ void load8<bf16>(const bf16* p, float (&x)[8]) {
+  const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[2 * i] = __uint_as_float(w[i] << 16), x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+}
+template <>
+__device__ __forceinline__ void load8<float>(const float* p, float (&x)[8]) {
+  const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+  x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+}
+__device__ __forceinline__ void store8(bf16* p, const float (&x)[8]) {
+  *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
+}
+__device__ __forceinline__ void store8(float* p, const float (&x)[8]) {
+  reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
+  reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
 }
 
-// One CTA per (page unit, KV head, K or V), then one per token row for the queries.
+// (x, y) = (x cos - y sin, y cos + x sin), eight columns of the two halves.
+__device__ __forceinline__ void rotate8(float (&x)[8], float (&y)[8], const float (&c)[8], const float (&s)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float a = x[i] * c[i] - y[i] * s[i];
+    y[i] = y[i] * c[i] + x[i] * s[i];
+    x[i] = a;
+  }
+}
+
+__device__ __forceinline__ uint2 code8(const float (&x)[8], float inv) {
+  uint32_t w[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+    w[h] = e4m3x2_from_f32(x[4 * h] * inv, x[4 * h + 1] * inv) |
+           static_cast<uint32_t>(e4m3x2_from_f32(x[4 * h + 2] * inv, x[4 * h + 3] * inv)) << 16;
+  return make_uint2(w[0], w[1]);
+}
+
+// The new scale of a page from its new rows' maximum (over this thread's part); every thread gets it.
+__device__ __forceinline__ float page_scale(float amax, bool keeps, float s_old, float* red) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = amax;
+  __syncthreads();
+  amax = red[0];
+  for (int w = 1; w < static_cast<int>(blockDim.x >> 5); ++w) amax = fmaxf(amax, red[w]);
+  const float s = pow2f(scale_exponent(amax));
+  return keeps && s_old > s ? s_old : s;
+}
+
 template <typename T, typename TT>
-__global__ void __launch_bounds__(128) paged_append_kernel(const PagedAppendArgs a) {
-  __shared__ float red[4];
+__global__ void __launch_bounds__(512) paged_append_kernel(const PagedAppendArgs a) {
+  __shared__ float red[16];
   pdl_trigger();
   pdl_wait();
-  const int hd = a.hd;
+  const int hd = a.hd, half = hd >> 1, tid = threadIdx.x;
   const int kv_blocks = a.n_units * a.hkv * 2;
-  if (static_cast<int>(blockIdx.x) >= kv_blocks) {  // queries
-    const int tok = blockIdx.x - kv_blocks;
-    const PagedReq r = a.reqs[paged_req_of(a.reqs, a.n, tok)];
-    const int pos = r.start + tok - r.tok0;
-    const T* src = static_cast<const T*>(a.q_in) + static_cast<size_t>(tok) * a.ldq;
-    T* dst = static_cast<T*>(a.q_out) + static_cast<size_t>(tok) * a.hq * hd;
-    for (int i = threadIdx.x; i < a.hq * hd; i += blockDim.x)
-      dst[i] = from_f<T>(new_value<T, TT>(src + i / hd * hd, i % hd, hd, true, a, pos));
+  const TT* cos_t = static_cast<const TT*>(a.cos);
+  const TT* sin_t = static_cast<const TT*>(a.sin);
+
+  if (static_cast<int>(blockIdx.x) >= kv_blocks) {  // ---- queries
+    const PagedPageUnit u = a.q_units[blockIdx.x - kv_blocks];  // (request, first token of it)
+    const PagedReq r = a.reqs[u.req];
+    const int lanes = half >> 3;                       // threads to a head row: 8 columns of each half
+    const int groups = blockDim.x / lanes, g = tid / lanes, d = (tid % lanes) * 8;
+    const int n_tok = min(kPagedQTokens, r.rows - u.slot);
+    const int split = max(1, groups / n_tok);          // groups to a token, a share of its heads each
+    const int step = groups / split;
+    if (g >= step * split) return;
+    for (int t = g / split; t < n_tok; t += step) {
+      const int tok = r.tok0 + u.slot + t;
+      const size_t at = static_cast<size_t>(r.start + u.slot + t) * half + d;
+      float c[8], s[8];
+      load8<TT>(cos_t + at, c);
+      load8<TT>(sin_t + at, s);
+      const T* src = static_cast<const T*>(a.q_in) + static_cast<size_t>(tok) * a.ldq + d;
+      T* dst = static_cast<T*>(a.q_out) + static_cast<size_t>(tok) * a.hq * hd + d;
+#pragma unroll 4
+      for (int h = g % split; h < a.hq; h += split) {
+        float x[8], y[8];
+        load8<T>(src + h * hd, x);
+        load8<T>(src + h * hd + half, y);
+        rotate8(x, y, c, s);
+        store8(dst + h * hd, x);
+        store8(dst + h * hd + half, y);
+      }
+    }
     return;
   }
+
+  // ---- a page's keys or values of one head
   const int is_v = blockIdx.x & 1, head = (blockIdx.x >> 1) % a.hkv;
   const PagedPageUnit u = a.units[(blockIdx.x >> 1) / a.hkv];
   const PagedReq r = a.reqs[u.req];
@@ -79,31 +150,75 @@ __global__ void __launch_bounds__(128) paged_append_kernel(const PagedAppendArgs
   const int ld = is_v ? a.ldv : a.ldk;
   const T* src = static_cast<const T*>(is_v ? a.v_in : a.k_in) +
                  static_cast<size_t>(r.tok0 + base + w0 - r.start) * ld + head * hd;
-  const int nw = (w1 - w0) * hd, pos0 = base + w0;
-
-  float amax = 0.f;
-  for (int i = threadIdx.x; i < nw; i += blockDim.x)
-    amax = fmaxf(amax, finite_abs(new_value<T, TT>(src + static_cast<size_t>(i / hd) * ld, i % hd, hd, !is_v, a, pos0 + i / hd)));
-  for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = amax;
-  const float s_old = *scale;
-  __syncthreads();
-  amax = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  const int n_rows = w1 - w0;
   const bool keeps = w0 > 0 || live > w1;  // rows below w0 held values: start <= live
-  float s = pow2f(scale_exponent(amax));
-  if (keeps && s_old > s) s = s_old;
-  const float inv = 1.f / s;
-  if (threadIdx.x == 0) *scale = s;
-  for (int i = threadIdx.x; i < nw; i += blockDim.x) {
-    const float x = new_value<T, TT>(src + static_cast<size_t>(i / hd) * ld, i % hd, hd, !is_v, a, pos0 + i / hd);
-    codes[w0 * hd + i] = static_cast<uint8_t>(e4m3x2_from_f32(x * inv, 0.f) & 0xFF);
+  const float s_old = *scale;
+  float s;
+  if (is_v) {
+    const int per = hd >> 3, items = n_rows * per;  // chunks: at most four a thread (page_size * hd / 8 <= 4 blockDim)
+    float x[4][8], amax = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int i = tid + j * blockDim.x;
+      if (i < items) load8<T>(src + static_cast<size_t>(i / per) * ld + (i % per) * 8, x[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (tid + j * static_cast<int>(blockDim.x) < items)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) amax = fmaxf(amax, finite_abs(x[j][e]));
+    s = page_scale(amax, keeps, s_old, red);
+    const float inv = 1.f / s;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int i = tid + j * blockDim.x;
+      if (i < items) *reinterpret_cast<uint2*>(codes + w0 * hd + i * 8) = code8(x[j], inv);
+    }
+  } else {
+    const int per = half >> 3, items = n_rows * per;  // chunk pairs: at most two a thread
+    float x[2][8], y[2][8], amax = 0.f;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int i = tid + j * blockDim.x;
+      if (i < items) {
+        const T* p = src + static_cast<size_t>(i / per) * ld + (i % per) * 8;
+        load8<T>(p, x[j]);
+        load8<T>(p + half, y[j]);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int i = tid + j * blockDim.x;
+      if (i < items) {
+        float c[8], sn[8];
+        const size_t at = static_cast<size_t>(base + w0 + i / per) * half + (i % per) * 8;
+        load8<TT>(cos_t + at, c);
+        load8<TT>(sin_t + at, sn);
+        rotate8(x[j], y[j], c, sn);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fmaxf(finite_abs(x[j][e]), finite_abs(y[j][e])));
+      }
+    }
+    s = page_scale(amax, keeps, s_old, red);
+    const float inv = 1.f / s;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int i = tid + j * blockDim.x;
+      if (i < items) {
+        uint8_t* dst = codes + (w0 + i / per) * hd + (i % per) * 8;
+        *reinterpret_cast<uint2*>(dst) = code8(x[j], inv);
+        *reinterpret_cast<uint2*>(dst + half) = code8(y[j], inv);
+      }
+    }
   }
-  if (keeps && s != s_old) {
+  if (tid == 0) *scale = s;
+  if (keeps && s != s_old) {  // kept rows, four codes at a time
     const float f = s_old / s;
-    const int n0 = w0 * hd, n1 = max(live - w1, 0) * hd;
-    for (int i = threadIdx.x; i < n0 + n1; i += blockDim.x) {
-      uint8_t* c = codes + (i < n0 ? i : w1 * hd + i - n0);
-      *c = static_cast<uint8_t>(e4m3x2_from_f32(f32x2_from_e4m3x2(*c).x * f, 0.f) & 0xFF);
+    const int n0 = w0 * hd / 4, n1 = max(live - w1, 0) * hd / 4;
+    for (int i = tid; i < n0 + n1; i += blockDim.x) {
+      uint32_t* c = reinterpret_cast<uint32_t*>(codes) + (i < n0 ? i : w1 * hd / 4 + i - n0);
+      const float2 lo = f32x2_from_e4m3x2(static_cast<uint16_t>(*c)), hi = f32x2_from_e4m3x2(static_cast<uint16_t>(*c >> 16));
+      *c = e4m3x2_from_f32(lo.x * f, lo.y * f) | static_cast<uint32_t>(e4m3x2_from_f32(hi.x * f, hi.y * f)) << 16;
     }
   }
 }
@@ -111,11 +226,12 @@ __global__ void __launch_bounds__(128) paged_append_kernel(const PagedAppendArgs
 }  // namespace
 
 int launch_paged_append(const PagedAppendArgs& a, int dtype, cudaStream_t s) {
-  const int grid = a.n_units * a.hkv * 2 + (a.q_in != nullptr ? a.total_rows : 0);
+  const int grid = a.n_units * a.hkv * 2 + (a.q_in != nullptr ? a.n_q_units : 0);
+  const int block = std::max(64, std::min(512, a.page_size * 4));  // two chunk pairs of a full page a thread at head_dim 128
   if (dtype == 1)
-    return a.table_f32 ? launch_k(paged_append_kernel<bf16, float>, dim3(grid), dim3(128), 0, s, a)
-                       : launch_k(paged_append_kernel<bf16, bf16>, dim3(grid), dim3(128), 0, s, a);
-  return launch_k(paged_append_kernel<float, float>, dim3(grid), dim3(128), 0, s, a);
+    return a.table_f32 ? launch_k(paged_append_kernel<bf16, float>, dim3(grid), dim3(block), 0, s, a)
+                       : launch_k(paged_append_kernel<bf16, bf16>, dim3(grid), dim3(block), 0, s, a);
+  return launch_k(paged_append_kernel<float, float>, dim3(grid), dim3(block), 0, s, a);
 }
 
 }  // namespace fdllm
