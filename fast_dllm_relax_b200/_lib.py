@@ -97,6 +97,7 @@ SIGNATURES: dict[str, tuple] = {
                                 _P, _I, _P, _I, _P, _I, _P, _P, _I, _P, _P]),
     "fdllm_paged_attention": (_I, [_P, ctypes.POINTER(FdllmPagedCache), _I, ctypes.POINTER(FdllmPagedPlan), _P, _P, _I,
                                    _P, _I, ctypes.c_float, _P, _P]),
+    "fdllm_forward_paged": (_I, [_P, ctypes.POINTER(FdllmPagedCache), ctypes.POINTER(FdllmPagedPlan), _P, _P, _I, _P, _P, _P]),
     "fdllm_logprobs": (_I, [_P, _P, _I, _I, _I, ctypes.c_longlong, _P, _I, _P, _P, _P, _P, _P]),
 }
 

@@ -32,13 +32,15 @@ import numpy as np
 import torch
 
 from .engine import Engine
+from .paged import PagedPool
 
 
 @dataclasses.dataclass
 class _Cache:
-    k: torch.Tensor
-    v: torch.Tensor
+    k: torch.Tensor | None  # contiguous caches, or
+    v: torch.Tensor | None
     prefix_len: int = 0
+    pages: list[int] | None = None  # the request's pages of a PagedPool
 
     @property
     def capacity(self) -> int:
@@ -63,7 +65,7 @@ def _id_tensor(seqs, n: int, dev) -> torch.Tensor:
 
 def request_program(engine: Engine, prompt_ids: Sequence[int], *, max_new_tokens: int, block_size: int,
                     small_block_size: int, threshold: float, use_block_cache: bool, mask_id: int,
-                    stop_token: int | None, stats: dict) -> Generator:
+                    stop_token: int | None, stats: dict, pool: PagedPool | None = None) -> Generator:
     """One request's decode loop (runtime.py:591-880, greedy); returns its continuation."""
     if max_new_tokens < 0:
         raise ValueError("max_new_tokens must be non-negative.")
@@ -75,6 +77,10 @@ def request_program(engine: Engine, prompt_ids: Sequence[int], *, max_new_tokens
     kv_valid = False
 
     def new_cache() -> _Cache:
+        if pool is not None:  # pages are taken as rows are written; a rebuilt prefix takes its own again
+            if cache is not None:
+                pool.release(cache.pages)
+            return _Cache(None, None, 0, [])
         k, v = engine.new_cache(cap)
         return _Cache(k, v, 0)
 
@@ -177,9 +183,11 @@ def request_program(engine: Engine, prompt_ids: Sequence[int], *, max_new_tokens
 def generate_batch(engine: Engine, prompts: Sequence[Sequence[int]], *, max_new_tokens: int,
                    block_size: int = 32, small_block_size: int = 8, threshold: float = 0.9,
                    use_block_cache: bool = False, mask_id: int, stop_token: int | None = None,
-                   timing: dict | None = None) -> tuple[list[list[int]], list[dict]]:
+                   timing: dict | None = None, pool: PagedPool | None = None) -> tuple[list[list[int]], list[dict]]:
     """Decode every prompt; returns (continuations, per-request statistics).  `timing`, when a
-    dict, receives total_ms and prefill_ms (the prefix-cache builds), measured with CUDA events."""
+    dict, receives total_ms and prefill_ms (the prefix-cache builds), measured with CUDA events.
+    `pool`: keep the requests' keys and values in its paged 8-bit cache (fdllm_forward_paged) instead of one
+    bf16 cache a request; its pages come back when a request is done."""
     if block_size != engine.cfg.bd_size:
         raise ValueError("block_size must equal the model's bd_size")
     dev = engine.device
@@ -187,7 +195,7 @@ def generate_batch(engine: Engine, prompts: Sequence[Sequence[int]], *, max_new_
     progs = [request_program(engine, p, max_new_tokens=max_new_tokens, block_size=block_size,
                              small_block_size=small_block_size, threshold=threshold,
                              use_block_cache=use_block_cache, mask_id=mask_id, stop_token=stop_token,
-                             stats=st) for p, st in zip(prompts, stats)]
+                             stats=st, pool=pool) for p, st in zip(prompts, stats)]
     results: list[list[int] | None] = [None] * len(progs)
     pending: dict[int, tuple] = {}
 
@@ -197,6 +205,20 @@ def generate_batch(engine: Engine, prompts: Sequence[Sequence[int]], *, max_new_
         except StopIteration as stop:
             results[i] = list(stop.value)
             pending.pop(i, None)
+            for pages in held.pop(i, ()):
+                pool.release(pages)
+
+    held: dict[int, list] = {}  # page lists of the requests (a pool's pages go back when one is done)
+
+    def paged_forward(ops, x, rows, start, live, causal_block, hidden):
+        """One forward of several requests over the pool's cache, their pages extended first."""
+        for i, op, n, s, lv in zip([i for i, _ in ops], [op for _, op in ops], rows, start, live):
+            pages = op[1].pages
+            if all(p is not pages for p in held.setdefault(i, [])):
+                held[i].append(pages)
+            pool.grow(pages, max(s + n, lv))
+        plan = engine.paged_plan(rows, start, live, page_size=pool.cache.page_size, causal_block=causal_block)
+        return engine.forward_paged(x, pool.cache, plan, pool.table([op[1].pages for _, op in ops]), hidden=hidden)
 
     ev = []  # (start, end) CUDA event pairs around prefix-cache builds
     staging = None  # pinned host buffer of a step's token ids and unmask descriptors
@@ -214,8 +236,13 @@ def generate_batch(engine: Engine, prompts: Sequence[Sequence[int]], *, max_new_
                 ev.append((torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)))
                 ev[-1][0].record()
             ids_all = _id_tensor([pending[i][2] for i in pre], sum(len(pending[i][2]) for i in pre), dev)
-            engine.build_prefix_cache_batch(engine.embed(ids_all), [(pending[i][1].k, pending[i][1].v) for i in pre],
-                                            [len(pending[i][2]) for i in pre])
+            if pool is not None:
+                n_pre = [len(pending[i][2]) for i in pre]
+                paged_forward([(i, pending[i]) for i in pre], engine.embed(ids_all), n_pre, [0] * len(pre), [0] * len(pre),
+                              block_size, False)
+            else:
+                engine.build_prefix_cache_batch(engine.embed(ids_all), [(pending[i][1].k, pending[i][1].v) for i in pre],
+                                                [len(pending[i][2]) for i in pre])
             if timing is not None:
                 ev[-1][1].record()
             for i in pre:
@@ -246,7 +273,14 @@ def generate_batch(engine: Engine, prompts: Sequence[Sequence[int]], *, max_new_
                              attend_rel=attend_rel))
             o += rows
         up = staging[:need].to(dev, non_blocking=True)
-        hidden = engine.forward_cached_batch(engine.embed(up[:n_ids]), reqs)
+        if pool is not None:
+            # a partial step rewrites rows inside a block whose other rows are cached: live reaches its end
+            start = [r["prefix_len"] + r["write_rel"] for r in reqs]
+            live = [max(s, r["prefix_len"] + (r["attend_rel"] if r["write_rel"] or r["rows"] < r["attend_rel"] else 0))
+                    for s, r in zip(start, reqs)]
+            hidden = paged_forward(steps, engine.embed(up[:n_ids]), [r["rows"] for r in reqs], start, live, 0, True)
+        else:
+            hidden = engine.forward_cached_batch(engine.embed(up[:n_ids]), reqs)
         cid, cmax = engine.confidence(hidden)
         dec = engine.unmask_batch(cid, cmax, up[n_ids:].view(len(steps), 5), threshold).cpu().numpy()
         for j, (i, op) in enumerate(steps):

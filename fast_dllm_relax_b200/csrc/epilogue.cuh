@@ -230,6 +230,11 @@ __device__ void gemm_epilogue(const GemmArgs& g, float* acc, int nt, int tok0, i
         Chunk<T> o;
         float x[V];
         ld_acc<V>(acc + t * 128 + f0, x);
+        if (e.bias != nullptr) {
+          const Chunk<T> bias = ld_const_chunk(static_cast<const T*>(e.bias) + F0);
+#pragma unroll
+          for (int v = 0; v < V; ++v) x[v] += to_f<T>(bias.e[v]);
+        }
 #pragma unroll
         for (int v = 0; v < V; v += 2) set_pair<T>(&o.e[v], x[v], x[v + 1]);
         st_chunk(out + (size_t)tok * e.ld_out + F0, o);

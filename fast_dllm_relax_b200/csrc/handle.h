@@ -210,6 +210,7 @@ struct fdllm_handle {
   DevBuf<float> attn_part, attn_part_lse;  // tcgen05 key-split partials
   DevBuf<float> persist_part;               // persistent-GEMM split-K partial tiles
   DevBuf<unsigned> persist_ctr;             // persistent-GEMM per-tile split counters (zero between launches)
+  DevBuf<uint8_t> paged_qkv;                // forward_paged: a layer's projected rows before RoPE
   DevBuf<float4> paged_part;                // paged attention: partials of tiles whose keys are split
   DevBuf<unsigned> paged_ctr;               //   and their arrived items (zero between launches)
   DevBuf<float4> logprob_part;              // log-probability partials of a row's parts
@@ -247,6 +248,16 @@ void release_step_graphs(fdllm_handle* h);
 int dense_forward(fdllm_handle* h, const void* x, const float* bias, int T, void* k, void* v, int cap, bool scratch,
                   void* out, cudaStream_t s);
 int cached_desc(fdllm_handle* h, const fdllm_request& r, int q_tok0, ReqDesc* d);
+// fdllm_paged_append / fdllm_paged_attention with the handle checked and locked, and the layer stack over them.
+int paged_append(fdllm_handle* h, const fdllm_paged_cache* cache, int layer, const fdllm_paged_plan* plan,
+                 const int32_t* plan_words, const int32_t* table, int table_ld, const void* q, int ldq, const void* k,
+                 int ldk, const void* v, int ldv, const float* rope_cos, const float* rope_sin, int rope_rows, void* q_out,
+                 cudaStream_t s);
+int paged_attention(fdllm_handle* h, const fdllm_paged_cache* cache, int layer, const fdllm_paged_plan* plan,
+                    const int32_t* plan_words, const int32_t* table, int table_ld, const void* q, int ldq, float scale,
+                    void* out, cudaStream_t s);
+int forward_paged(fdllm_handle* h, const fdllm_paged_cache* cache, const fdllm_paged_plan* plan, const int32_t* words,
+                  const int32_t* table, int table_ld, const void* x, void* out, cudaStream_t s);
 // 2D uint8 map of a paged cache's codes as rows of head_dim bytes, box one page (at most 64 rows), 128-byte
 // swizzle at head_dim 128.
 int make_page_map(CUtensorMap* map, const void* base, const fdllm_paged_cache* c, int kv_heads, int head_dim);

@@ -44,7 +44,7 @@ struct TokenMaps {
 };
 
 enum EpiKind : int {
-  kEpiStore = 0,      // out[t, f] = T(acc)
+  kEpiStore = 0,      // out[t, f] = T(acc), or T(acc + bias)
   kEpiQkvRope = 1,    // + bias, RoPE on q/k, q -> qout, k/v -> caches (per-token rows)
   kEpiResidual = 2,   // resid[t, f] = T(resid + T(acc))
   kEpiSiluMul = 3,    // paired gate/up slab: out[t, j] = T(T(silu(T(gate))) * T(up))
@@ -58,7 +58,7 @@ struct Epilogue {
   int layer;
   void* out;                // Store / SiluMul: [M, ld_out] in T; LogitsF32: float [M, ld_out]
   int ld_out;
-  const void* bias;         // QkvRope: [N] in T
+  const void* bias;         // QkvRope: [N] in T; Store: the same or null
   void* resid;              // Residual: [M, ld_resid] in T
   const void* resid_src;    // Residual: optional source of the residual (else resid); same layout
   float* ss_out;            // Residual: optional [M, ss_ld] sum of squares of each new row's 128-feature

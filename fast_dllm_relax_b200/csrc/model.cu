@@ -458,6 +458,44 @@ int fdllm::reserve_workspace(fdllm_handle* h, int M, int nreq, int max_l) {
   return FDLLM_OK;
 }
 
+// The second half of a layer (model/cuda.py:546-579): o projection += h, post-attention RMSNorm, gate_up with
+// SiLU * up, down projection += h.  The attention output is in h->attn.
+static int layer_tail(fdllm_handle* h, const LayerW& L, const Epilogue& base, int M, bool fuse_norm, bool fuse_norm_gu,
+                      cudaStream_t s) {
+  const fdllm_config& c = h->cfg;
+  Epilogue e = base;
+  e.kind = kEpiResidual;
+  e.resid = h->h.p;
+  e.ld_resid = c.hidden_size;
+  if (fuse_norm_gu) {  // leave the statistics of the post-attention RMSNorm
+    e.ss_out = h->ss.p;
+    e.ss_ld = c.hidden_size / 128;
+  }
+  FDLLM_TRY(run_gemm(h, L.o, h->attn.p, M, e, s));
+
+  e = base;
+  e.kind = kEpiSiluMul;
+  e.out = h->act.p;
+  e.ld_out = c.intermediate_size;
+  if (fuse_norm_gu) {
+    FDLLM_TRY(run_gemm(h, L.gu, h->h.p, M, e, s, L.ln2));
+  } else {
+    CUDA_TRY(launch_rmsnorm(h->h.p, L.ln2, h->xn.p, M, c.hidden_size, c.rms_norm_eps, h->dtype, s));
+    FDLLM_TRY(run_gemm(h, L.gu, h->xn.p, M, e, s));
+  }
+
+  e = base;
+  e.kind = kEpiResidual;
+  e.resid = h->h.p;
+  e.ld_resid = c.hidden_size;
+  if (fuse_norm) {  // leave the statistics of the next layer's input RMSNorm
+    e.ss_out = h->ss.p;
+    e.ss_ld = c.hidden_size / 128;
+  }
+  FDLLM_TRY(run_gemm(h, L.down, h->act.p, M, e, s));
+  return FDLLM_OK;
+}
+
 // ---- the layer stack ----------------------------------------------------------------------
 // x: [M, hidden] input embeddings; reqs: host descriptors (q_tok0 / n_q filled); bias: dense fp32
 // bias of request 0 (or null), causal_block: implicit block-causal mask when bias is null.
@@ -605,39 +643,52 @@ int fdllm::forward_core(fdllm_handle* h, const void* x, int M, std::vector<ReqDe
       CUDA_TRY(launch_attention(a, max_q, h->dtype, s));
     }
 
-    e = base;
-    e.kind = kEpiResidual;
-    e.resid = h->h.p;
-    e.ld_resid = c.hidden_size;
-    if (fuse_norm_gu) {  // leave the statistics of the post-attention RMSNorm
-      e.ss_out = h->ss.p;
-      e.ss_ld = c.hidden_size / 128;
-    }
-    FDLLM_TRY(run_gemm(h, L.o, h->attn.p, M, e, s));
-
-    e = base;
-    e.kind = kEpiSiluMul;
-    e.out = h->act.p;
-    e.ld_out = c.intermediate_size;
-    if (fuse_norm_gu) {
-      FDLLM_TRY(run_gemm(h, L.gu, h->h.p, M, e, s, L.ln2));
-    } else {
-      CUDA_TRY(launch_rmsnorm(h->h.p, L.ln2, h->xn.p, M, c.hidden_size, c.rms_norm_eps, h->dtype, s));
-      FDLLM_TRY(run_gemm(h, L.gu, h->xn.p, M, e, s));
-    }
-
-    e = base;
-    e.kind = kEpiResidual;
-    e.resid = h->h.p;
-    e.ld_resid = c.hidden_size;
-    if (fuse_norm) {  // leave the statistics of the next layer's input RMSNorm
-      e.ss_out = h->ss.p;
-      e.ss_ld = c.hidden_size / 128;
-    }
-    FDLLM_TRY(run_gemm(h, L.down, h->act.p, M, e, s));
+    FDLLM_TRY(layer_tail(h, L, base, M, fuse_norm, fuse_norm_gu, s));
   }
   // out == null (build_prefix_cache): the final hidden states are not needed; xn is free by now.
   CUDA_TRY(launch_rmsnorm(h->h.p, h->final_norm, out ? out : h->xn.p, M, c.hidden_size, c.rms_norm_eps, h->dtype, s));
+  return FDLLM_OK;
+}
+
+// The layer stack over a paged 8-bit cache: the qkv projection leaves its rows as they are (bias added), the
+// append rotates and codes them into the layer's pages, the attention reads the pages.
+int fdllm::forward_paged(fdllm_handle* h, const fdllm_paged_cache* cache, const fdllm_paged_plan* plan,
+                         const int32_t* words, const int32_t* table, int table_ld, const void* x, void* out,
+                         cudaStream_t s) {
+  const fdllm_config& c = h->cfg;
+  const int M = plan->total_rows, q_cols = c.num_attention_heads * c.head_dim, kv_cols = c.num_key_value_heads * c.head_dim;
+  const int ld = q_cols + 2 * kv_cols;
+  FDLLM_TRY(ensure_ws(h, M, 1));
+  FDLLM_TRY(h->paged_qkv.ensure(static_cast<size_t>(M) * ld * h->esz));
+  const bool fuse_norm = h->dtype == FDLLM_BFLOAT16 && M <= 64 && c.hidden_size <= 2560;
+  const bool fuse_norm_gu = fuse_norm && M <= h->tune.gu_fused_rows;
+  const uint8_t* qkv = h->paged_qkv.p;
+  Epilogue base{};
+  for (int l = 0; l < c.num_hidden_layers; ++l) {
+    const LayerW& L = h->layers[l];
+    const void* layer_in = l == 0 ? x : h->h.p;
+    Epilogue e = base;
+    e.kind = kEpiStore;
+    e.layer = l;
+    e.bias = L.qkv_b;
+    e.out = h->paged_qkv.p;
+    e.ld_out = ld;
+    if (fuse_norm && l > 0) {
+      FDLLM_TRY(run_gemm(h, L.qkv, layer_in, M, e, s, L.ln1));
+    } else {
+      CUDA_TRY(launch_rmsnorm(layer_in, L.ln1, h->xn.p, M, c.hidden_size, c.rms_norm_eps, h->dtype, s,
+                              l == 0 ? h->h.p : nullptr));
+      FDLLM_TRY(run_gemm(h, L.qkv, h->xn.p, M, e, s));
+    }
+    FDLLM_TRY(paged_append(h, cache, l, plan, words, table, table_ld, qkv, ld, qkv + q_cols * h->esz, ld,
+                           qkv + (q_cols + kv_cols) * h->esz, ld, nullptr, nullptr, 0, h->q.p, s));
+    FDLLM_TRY(paged_attention(h, cache, l, plan, words, table, table_ld, h->q.p, q_cols,
+                              1.0f / std::sqrt(static_cast<float>(c.head_dim)), h->attn.p, s));
+    FDLLM_TRY(layer_tail(h, L, base, M, fuse_norm, fuse_norm_gu, s));
+  }
+  // out == null (a prefix build): the final hidden states are not needed
+  if (out != nullptr)
+    CUDA_TRY(launch_rmsnorm(h->h.p, h->final_norm, out, M, c.hidden_size, c.rms_norm_eps, h->dtype, s));
   return FDLLM_OK;
 }
 
@@ -757,6 +808,7 @@ int fdllm_destroy(fdllm_handle* h) {
   for (auto* b : {&h->conf_part, &h->tmp_maxp, &h->ss, &h->dec.cmax}) b->release();
   h->persist_part.release();
   h->persist_ctr.release();
+  h->paged_qkv.release();
   h->paged_part.release();
   h->paged_ctr.release();
   h->logprob_part.release();

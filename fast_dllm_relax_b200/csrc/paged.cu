@@ -175,6 +175,118 @@ int plan_items(const fdllm_handle* h, const std::vector<PagedReq>& reqs, int cau
 
 }  // namespace
 
+int fdllm::paged_append(fdllm_handle* h, const fdllm_paged_cache* cache, int layer, const fdllm_paged_plan* plan,
+                        const int32_t* plan_words, const int32_t* table, int table_ld, const void* q, int ldq,
+                        const void* k, int ldk, const void* v, int ldv, const float* rope_cos, const float* rope_sin,
+                        int rope_rows, void* q_out, cudaStream_t s) {
+  size_t codes, scales;
+  FDLLM_TRY(check_paged(h, cache, layer, plan, plan_words, table, table_ld, &codes, &scales));
+  if ((rope_cos == nullptr) != (rope_sin == nullptr)) return fail(FDLLM_ERR_INVALID, "rope_cos and rope_sin go together");
+  const int have = rope_cos != nullptr ? rope_rows : h->cfg.max_positions;
+  if (plan->max_position > have)
+    return fail(FDLLM_ERR_INVALID, "RoPE positions reach " + std::to_string(plan->max_position) + "; the tables have " +
+                                       std::to_string(have) + " rows");
+  if (rope_cos != nullptr && (!aligned16(rope_cos) || !aligned16(rope_sin)))
+    return fail(FDLLM_ERR_INVALID, "RoPE tables must be 16-byte aligned");
+  if (plan->total_rows == 0) return FDLLM_OK;
+  const fdllm_config& c = h->cfg;
+  if ((q == nullptr) != (q_out == nullptr)) return fail(FDLLM_ERR_INVALID, "q and q_out go together");
+  if (q != nullptr) {
+    FDLLM_TRY(check_rows(h, "q", q, ldq, c.num_attention_heads * c.head_dim));
+    FDLLM_TRY(check_rows(h, "q_out", q_out, c.num_attention_heads * c.head_dim, c.num_attention_heads * c.head_dim));
+  }
+  FDLLM_TRY(check_rows(h, "k", k, ldk, c.num_key_value_heads * c.head_dim));
+  FDLLM_TRY(check_rows(h, "v", v, ldv, c.num_key_value_heads * c.head_dim));
+  PagedAppendArgs a{};
+  a.reqs = reinterpret_cast<const PagedReq*>(plan_words);
+  a.units = reinterpret_cast<const PagedPageUnit*>(plan_words + plan->priv[kPagedPageOff]);
+  a.n_units = plan->priv[kPagedPageUnits];
+  a.q_units = reinterpret_cast<const PagedPageUnit*>(plan_words + plan->priv[kPagedQOff]);
+  a.n_q_units = plan->priv[kPagedQUnits];
+  a.n = plan->n;
+  a.total_rows = plan->total_rows;
+  a.table = table;
+  a.table_ld = table_ld;
+  a.k = static_cast<uint8_t*>(cache->k) + codes;
+  a.v = static_cast<uint8_t*>(cache->v) + codes;
+  a.k_scale = cache->k_scale + scales;
+  a.v_scale = cache->v_scale + scales;
+  a.pages = cache->pages;
+  a.page_size = cache->page_size;
+  a.hq = c.num_attention_heads;
+  a.hkv = c.num_key_value_heads;
+  a.hd = c.head_dim;
+  a.q_in = q;
+  a.k_in = k;
+  a.v_in = v;
+  a.ldq = ldq;
+  a.ldk = ldk;
+  a.ldv = ldv;
+  a.table_f32 = rope_cos != nullptr || h->dtype == FDLLM_FLOAT32;
+  a.cos = rope_cos != nullptr ? static_cast<const void*>(rope_cos) : h->rope_cos.p;
+  a.sin = rope_sin != nullptr ? static_cast<const void*>(rope_sin) : h->rope_sin.p;
+  a.q_out = q_out;
+  a.err = h->err.p;
+  CUDA_TRY(launch_paged_append(a, h->dtype, s));
+  return FDLLM_OK;
+}
+
+int fdllm::paged_attention(fdllm_handle* h, const fdllm_paged_cache* cache, int layer, const fdllm_paged_plan* plan,
+                           const int32_t* plan_words, const int32_t* table, int table_ld, const void* q, int ldq,
+                           float scale, void* out, cudaStream_t s) {
+  size_t codes, scales;
+  FDLLM_TRY(check_paged(h, cache, layer, plan, plan_words, table, table_ld, &codes, &scales));
+  if (!std::isfinite(scale)) return fail(FDLLM_ERR_INVALID, "scale must be finite");
+  if (plan->total_rows == 0) return FDLLM_OK;
+  const fdllm_config& c = h->cfg;
+  const int cols = c.num_attention_heads * c.head_dim;
+  FDLLM_TRY(check_rows(h, "q", q, ldq, cols));
+  FDLLM_TRY(check_rows(h, "out", out, cols, cols));
+  PagedAttnArgs a{};
+  a.reqs = reinterpret_cast<const PagedReq*>(plan_words);
+  a.n = plan->n;
+  a.total_rows = plan->total_rows;
+  a.table = table;
+  a.table_ld = table_ld;
+  a.k = static_cast<const uint8_t*>(cache->k) + codes;
+  a.v = static_cast<const uint8_t*>(cache->v) + codes;
+  a.k_scale = cache->k_scale + scales;
+  a.v_scale = cache->v_scale + scales;
+  a.pages = cache->pages;
+  a.page_size = cache->page_size;
+  while ((1 << a.page_shift) < a.page_size) ++a.page_shift;
+  a.hq = c.num_attention_heads;
+  a.hkv = c.num_key_value_heads;
+  a.hd = c.head_dim;
+  a.causal_block = plan->causal_block;
+  a.q = q;
+  a.ldq = ldq;
+  a.scale = scale;
+  a.out = out;
+  a.err = h->err.p;
+  if (h->dtype != FDLLM_BFLOAT16) {
+    CUDA_TRY(launch_paged_attention_simt(a, s));
+    return FDLLM_OK;
+  }
+  FDLLM_TRY(h->paged_part.ensure(plan->priv[kPagedParts]));
+  FDLLM_TRY(ensure_counters(&h->paged_ctr, plan->priv[kPagedTiles], s));
+  CUtensorMap tm_k, tm_v;
+  FDLLM_TRY(make_page_map(&tm_k, cache->k, cache, c.num_key_value_heads, c.head_dim));
+  FDLLM_TRY(make_page_map(&tm_v, cache->v, cache, c.num_key_value_heads, c.head_dim));
+  a.layer_row = static_cast<int>(codes / c.head_dim);
+  a.part = h->paged_part.p;
+  a.arrived = h->paged_ctr.p;
+  for (int k = 0; k < kPagedClasses; ++k) {
+    if (plan->priv[kPagedItems + k] == 0) continue;
+    a.items = reinterpret_cast<const PagedItem*>(plan_words + plan->priv[kPagedItemOff + k]);
+    const int n = plan->priv[kPagedItems + k];
+    CUDA_TRY(c.head_dim != 128  ? launch_paged_attention_narrow(a, k + 1, n, tm_k, tm_v, s)
+             : k == kPagedWide ? launch_paged_attention_wide(a, n, tm_k, tm_v, s)
+                               : launch_paged_attention_tc(a, 16 * (k + 1), n, tm_k, tm_v, s));
+  }
+  return FDLLM_OK;
+}
+
 extern "C" {
 
 int fdllm_paged_plan_batch(fdllm_handle* h, const int32_t* rows, const int32_t* start, const int32_t* live, int n,
@@ -254,57 +366,9 @@ int fdllm_paged_append(fdllm_handle* h, const fdllm_paged_cache* cache, int laye
                        int rope_rows, void* q_out, void* stream) {
   return guarded([&]() -> int {
     FDLLM_TRY(check_handle(h));
-    size_t codes, scales;
-    FDLLM_TRY(check_paged(h, cache, layer, plan, plan_words, table, table_ld, &codes, &scales));
-    if ((rope_cos == nullptr) != (rope_sin == nullptr)) return fail(FDLLM_ERR_INVALID, "rope_cos and rope_sin go together");
-    const int have = rope_cos != nullptr ? rope_rows : h->cfg.max_positions;
-    if (plan->max_position > have)
-      return fail(FDLLM_ERR_INVALID, "RoPE positions reach " + std::to_string(plan->max_position) + "; the tables have " +
-                                         std::to_string(have) + " rows");
-    if (rope_cos != nullptr && (!aligned16(rope_cos) || !aligned16(rope_sin)))
-      return fail(FDLLM_ERR_INVALID, "RoPE tables must be 16-byte aligned");
-    if (plan->total_rows == 0) return FDLLM_OK;
-    const fdllm_config& c = h->cfg;
-    if ((q == nullptr) != (q_out == nullptr)) return fail(FDLLM_ERR_INVALID, "q and q_out go together");
-    if (q != nullptr) {
-      FDLLM_TRY(check_rows(h, "q", q, ldq, c.num_attention_heads * c.head_dim));
-      FDLLM_TRY(check_rows(h, "q_out", q_out, c.num_attention_heads * c.head_dim, c.num_attention_heads * c.head_dim));
-    }
-    FDLLM_TRY(check_rows(h, "k", k, ldk, c.num_key_value_heads * c.head_dim));
-    FDLLM_TRY(check_rows(h, "v", v, ldv, c.num_key_value_heads * c.head_dim));
-    PagedAppendArgs a{};
-    a.reqs = reinterpret_cast<const PagedReq*>(plan_words);
-    a.units = reinterpret_cast<const PagedPageUnit*>(plan_words + plan->priv[kPagedPageOff]);
-    a.n_units = plan->priv[kPagedPageUnits];
-    a.q_units = reinterpret_cast<const PagedPageUnit*>(plan_words + plan->priv[kPagedQOff]);
-    a.n_q_units = plan->priv[kPagedQUnits];
-    a.n = plan->n;
-    a.total_rows = plan->total_rows;
-    a.table = table;
-    a.table_ld = table_ld;
-    a.k = static_cast<uint8_t*>(cache->k) + codes;
-    a.v = static_cast<uint8_t*>(cache->v) + codes;
-    a.k_scale = cache->k_scale + scales;
-    a.v_scale = cache->v_scale + scales;
-    a.pages = cache->pages;
-    a.page_size = cache->page_size;
-    a.hq = c.num_attention_heads;
-    a.hkv = c.num_key_value_heads;
-    a.hd = c.head_dim;
-    a.q_in = q;
-    a.k_in = k;
-    a.v_in = v;
-    a.ldq = ldq;
-    a.ldk = ldk;
-    a.ldv = ldv;
-    a.table_f32 = rope_cos != nullptr || h->dtype == FDLLM_FLOAT32;
-    a.cos = rope_cos != nullptr ? static_cast<const void*>(rope_cos) : h->rope_cos.p;
-    a.sin = rope_sin != nullptr ? static_cast<const void*>(rope_sin) : h->rope_sin.p;
-    a.q_out = q_out;
     std::lock_guard<std::mutex> lock(h->mu);
-    a.err = h->err.p;
-    CUDA_TRY(launch_paged_append(a, h->dtype, static_cast<cudaStream_t>(stream)));
-    return FDLLM_OK;
+    return paged_append(h, cache, layer, plan, plan_words, table, table_ld, q, ldq, k, ldk, v, ldv, rope_cos, rope_sin,
+                        rope_rows, q_out, static_cast<cudaStream_t>(stream));
   });
 }
 
@@ -313,59 +377,28 @@ int fdllm_paged_attention(fdllm_handle* h, const fdllm_paged_cache* cache, int l
                           float scale, void* out, void* stream) {
   return guarded([&]() -> int {
     FDLLM_TRY(check_handle(h));
-    size_t codes, scales;
-    FDLLM_TRY(check_paged(h, cache, layer, plan, plan_words, table, table_ld, &codes, &scales));
-    if (!std::isfinite(scale)) return fail(FDLLM_ERR_INVALID, "scale must be finite");
-    if (plan->total_rows == 0) return FDLLM_OK;
-    const fdllm_config& c = h->cfg;
-    const int cols = c.num_attention_heads * c.head_dim;
-    FDLLM_TRY(check_rows(h, "q", q, ldq, cols));
-    FDLLM_TRY(check_rows(h, "out", out, cols, cols));
-    PagedAttnArgs a{};
-    a.reqs = reinterpret_cast<const PagedReq*>(plan_words);
-    a.n = plan->n;
-    a.total_rows = plan->total_rows;
-    a.table = table;
-    a.table_ld = table_ld;
-    a.k = static_cast<const uint8_t*>(cache->k) + codes;
-    a.v = static_cast<const uint8_t*>(cache->v) + codes;
-    a.k_scale = cache->k_scale + scales;
-    a.v_scale = cache->v_scale + scales;
-    a.pages = cache->pages;
-    a.page_size = cache->page_size;
-    while ((1 << a.page_shift) < a.page_size) ++a.page_shift;
-    a.hq = c.num_attention_heads;
-    a.hkv = c.num_key_value_heads;
-    a.hd = c.head_dim;
-    a.causal_block = plan->causal_block;
-    a.q = q;
-    a.ldq = ldq;
-    a.scale = scale;
-    a.out = out;
     std::lock_guard<std::mutex> lock(h->mu);
-    a.err = h->err.p;
-    const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (h->dtype != FDLLM_BFLOAT16) {
-      CUDA_TRY(launch_paged_attention_simt(a, st));
-      return FDLLM_OK;
-    }
-    FDLLM_TRY(h->paged_part.ensure(plan->priv[kPagedParts]));
-    FDLLM_TRY(ensure_counters(&h->paged_ctr, plan->priv[kPagedTiles], st));
-    CUtensorMap tm_k, tm_v;
-    FDLLM_TRY(make_page_map(&tm_k, cache->k, cache, c.num_key_value_heads, c.head_dim));
-    FDLLM_TRY(make_page_map(&tm_v, cache->v, cache, c.num_key_value_heads, c.head_dim));
-    a.layer_row = static_cast<int>(codes / c.head_dim);
-    a.part = h->paged_part.p;
-    a.arrived = h->paged_ctr.p;
-    for (int k = 0; k < kPagedClasses; ++k) {
-      if (plan->priv[kPagedItems + k] == 0) continue;
-      a.items = reinterpret_cast<const PagedItem*>(plan_words + plan->priv[kPagedItemOff + k]);
-      const int n = plan->priv[kPagedItems + k];
-      CUDA_TRY(c.head_dim != 128  ? launch_paged_attention_narrow(a, k + 1, n, tm_k, tm_v, st)
-               : k == kPagedWide ? launch_paged_attention_wide(a, n, tm_k, tm_v, st)
-                                 : launch_paged_attention_tc(a, 16 * (k + 1), n, tm_k, tm_v, st));
-    }
-    return FDLLM_OK;
+    return paged_attention(h, cache, layer, plan, plan_words, table, table_ld, q, ldq, scale, out,
+                           static_cast<cudaStream_t>(stream));
+  });
+}
+
+int fdllm_forward_paged(fdllm_handle* h, const fdllm_paged_cache* cache, const fdllm_paged_plan* plan,
+                        const int32_t* plan_words, const int32_t* table, int table_ld, const void* x, void* out,
+                        void* stream) {
+  return guarded([&]() -> int {
+    FDLLM_TRY(check_handle(h));
+    size_t codes, scales;
+    FDLLM_TRY(check_paged(h, cache, 0, plan, plan_words, table, table_ld, &codes, &scales));
+    if (cache->layers != h->cfg.num_hidden_layers)
+      return fail(FDLLM_ERR_INVALID, "the paged cache has " + std::to_string(cache->layers) + " layers, the model " +
+                                         std::to_string(h->cfg.num_hidden_layers));
+    if (plan->max_position > h->cfg.max_positions)
+      return fail(FDLLM_ERR_INVALID, "RoPE positions exceed max_positions");
+    if (plan->total_rows == 0) return FDLLM_OK;
+    if (x == nullptr) return fail(FDLLM_ERR_INVALID, "null x");
+    std::lock_guard<std::mutex> lock(h->mu);
+    return forward_paged(h, cache, plan, plan_words, table, table_ld, x, out, static_cast<cudaStream_t>(stream));
   });
 }
 

@@ -391,6 +391,20 @@ class Engine:
             q.stride(0), self.cfg.head_dim ** -0.5 if scale is None else scale, out.data_ptr(), self._raw_stream()))
         return out
 
+    def forward_paged(self, x: torch.Tensor, cache: PagedCache, plan: PagedPlan, table: torch.Tensor,
+                      hidden: bool = True) -> torch.Tensor | None:
+        """The model over a paged cache (fdllm_forward_paged): embeddings x [total_rows, hidden] of the
+        plan's token rows -> hidden states, every layer's keys and values appended on the way.
+        hidden=False only builds the cache."""
+        self._paged(cache, plan, table, "forward_paged")
+        x2 = self._act(x, "forward_paged")
+        if x2.shape[0] != plan.total_rows:
+            raise ValueError(f"forward_paged: the plan has {plan.total_rows} rows, x {x2.shape[0]}")
+        out = torch.empty_like(x2) if hidden else None
+        _lib.check(self.lib.fdllm_forward_paged(self._h, cache.ref, plan.ref, plan.words_ptr, table.data_ptr(),
+                                                table.shape[1], x2.data_ptr(), _ptr(out), self._raw_stream()))
+        return out
+
     def generate(self, prompt_ids: Sequence[int], *, max_new_tokens: int, block_size: int = 32,
                  small_block_size: int = 8, threshold: float = 0.9, use_block_cache: bool = False, mask_id: int,
                  stop_token: int | None = None, timing: dict | None = None) -> tuple[list[int], dict]:

@@ -2,6 +2,7 @@
 `Engine.paged_attention` (the reference's caches are one contiguous buffer per request).
 
     cache = eng.new_paged_cache(pages, page_size=32)
+    pool = PagedPool(cache)                                   # free pages; pool.grow / release / table
     plan = eng.paged_plan(rows, start, page_size=32)          # one per step, shared by every layer
     q = eng.paged_append(cache, layer, plan, table, q, k, v)  # rotate, code, write
     o = eng.paged_attention(cache, layer, plan, table, q)
@@ -61,6 +62,38 @@ class PagedCache:
     @property
     def page_size(self) -> int:
         return int(self.k.shape[3])
+
+
+class PagedPool:
+    """The free pages of a cache.  Requests take pages as they grow and give them back when done."""
+
+    def __init__(self, cache: PagedCache):
+        self.cache = cache
+        self._free = list(range(cache.pages - 1, -1, -1))
+
+    @property
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def grow(self, pages: list[int], rows: int) -> None:
+        """Extend a request's page list to hold `rows` cache rows."""
+        need = -(-rows // self.cache.page_size) - len(pages)
+        if need > len(self._free):
+            raise MemoryError(f"paged cache: {need} pages needed, {len(self._free)} free")
+        pages.extend(self._free.pop() for _ in range(need))
+
+    def release(self, pages: list[int]) -> None:
+        self._free.extend(reversed(pages))
+        pages.clear()
+
+    def table(self, requests: list[list[int]]) -> torch.Tensor:
+        """int32 [n, columns] page table of several requests on the cache's device."""
+        width = max((len(p) for p in requests), default=0) or 1
+        host = torch.zeros((len(requests), width), dtype=torch.int32, pin_memory=self.cache.device.type == "cuda")
+        rows = host.numpy()
+        for i, p in enumerate(requests):
+            rows[i, :len(p)] = p
+        return host.to(self.cache.device, non_blocking=True)
 
 
 class PagedPlan:

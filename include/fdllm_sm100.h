@@ -305,6 +305,15 @@ FDLLM_API int fdllm_paged_attention(fdllm_handle* h, const fdllm_paged_cache* ca
                                     const fdllm_paged_plan* plan, const int32_t* plan_words, const int32_t* table,
                                     int table_ld, const void* q, int ldq, float scale, void* out, void* stream);
 
+/* The model over a paged cache (all its layers): x [total_rows, hidden] embeddings of the batch's token rows
+ * -> out [total_rows, hidden] after the final norm (NULL: only the cache is wanted, a prefix build).  Every
+ * layer appends its keys and values with the handle's RoPE tables and attends the pages; with causal_block =
+ * bd_size this is build_prefix_cache of many requests, with 0 their forward_cached (live = prefix + block for
+ * the partial form, which rewrites rows inside a block). */
+FDLLM_API int fdllm_forward_paged(fdllm_handle* h, const fdllm_paged_cache* cache, const fdllm_paged_plan* plan,
+                                  const int32_t* plan_words, const int32_t* table, int table_ld, const void* x, void* out,
+                                  void* stream);
+
 /* Log probabilities of given tokens, with entropy and top alternatives, from logits [rows, vocab]
  * (logits_dtype FDLLM_FLOAT32 or FDLLM_BFLOAT16, row stride ld elements).  The reference reduces
  * logits on the host (runners.py:877-881).  Per row, in fp32: lse = log sum exp(logits);
