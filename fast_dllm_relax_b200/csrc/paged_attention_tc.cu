@@ -153,15 +153,13 @@ struct Bars {
   uint64_t k_full[3], k_empty[3], v_full[3], v_empty[3];
   uint64_t q_ready, s_full, s_free, p_full, pv_done[2], o_final;
   uint32_t tmem;
-  int last;
   // of a stage's pages: log2 vs, 1 / vs, and ks over that of the first page of the 32 keys
   float4 scale[3][kKeys / 16];
   // x = S map + log2 vs - base: unscale ks of a column, for the first page of each 32 keys
   alignas(16) float map[3][4][N];
-  alignas(16) float unscale[N], base[N], delta[N], factor[N];
+  alignas(16) float base[N], delta[N], factor[N];
+  PagedRows<N> rows;
   float part[4][N];  // a warp's column maxima, at the end its column sums
-  int lim[N];
-  int out[N];        // (token, head) row of the output
 };
 template <int N>
 constexpr bool two_ctas() { return Cfg<N>::kBytes + static_cast<int>(sizeof(Bars<N>)) + 1024 <= 228 * 1024 / 2; }
@@ -213,7 +211,6 @@ __global__ void __launch_bounds__(kThreads, 2)
   pdl_trigger();
   pdl_wait();
   const PagedItem it = a.items[blockIdx.x];
-  const int G = a.hq / a.hkv;
   const int n_tiles = (it.key1 - it.key0 + kKeys - 1) / kKeys;
 
   if (warp < 4) set_registers<kRegsMisc, false>();
@@ -273,7 +270,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const float kg = __shfl_sync(0xffffffffu, ks_j, (32 * g) >> a.page_shift);
-        for (int n = lane; n < N; n += 32) b.map[st][g][n] = b.unscale[n] * kg;
+        for (int n = lane; n < N; n += 32) b.map[st][g][n] = b.rows.unscale[n] * kg;
       }
       mbar_arrive(&b.v_full[st]);
       __syncwarp();
@@ -326,68 +323,17 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
   } else if (warp >= 4) {
     set_registers<kRegsSoftmax, true>();
-    {
-      // queries: a warp a row, four head columns a lane, all loads in flight
-      constexpr int kQr = N / 8;
-      const int w8 = warp - 4;
-      // row / G and row % G from the first row's, by multiplication (small operands)
-      const unsigned inv_g = 0xFFFFFFFFu / G + 1;
-      const int g0 = it.row0 % G, tok_base = it.row0 / G;
-      uint2 raw[kQr];
-#pragma unroll
-      for (int i = 0; i < kQr; ++i) {
-        const int n = w8 + 8 * i;
-        const int t = G == 1 ? g0 + n : __umulhi(g0 + n, inv_g), h = g0 + n - t * G;
-        raw[i] = make_uint2(0u, 0u);
-        if (n < it.rows)
-          raw[i] = *reinterpret_cast<const uint2*>(static_cast<const bf16*>(a.q) +
-                                                   static_cast<size_t>(it.tok0 + tok_base + t) * a.ldq +
-                                                   static_cast<size_t>(it.head * G + h) * kHd + 4 * lane);
-      }
-#pragma unroll
-      for (int i = 0; i < kQr; ++i) {
-        const int n = w8 + 8 * i;
-        const uint2 u = raw[i];
-        const float x[4] = {__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xFFFF0000u), __uint_as_float(u.y << 16),
-                            __uint_as_float(u.y & 0xFFFF0000u)};
-        float m = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-        // exponent of m, kept where both the scale and its inverse are normal floats
-        const int e = min(max(static_cast<int>(__float_as_uint(m) >> 23) - 127, -110), 110);
-        const float up = m > 0.f ? __uint_as_float(static_cast<uint32_t>(127 + 7 - e) << 23) : 1.f;
-        uint32_t hi = 0, lo = 0;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float x0 = x[2 * h] * up, x1 = x[2 * h + 1] * up;
-          const uint16_t c = e4m3x2_from_f32(x0, x1);
-          const float2 r = f32x2_from_e4m3x2(c);
-          hi |= static_cast<uint32_t>(c) << (16 * h);
-          lo |= static_cast<uint32_t>(e4m3x2_from_f32(x0 - r.x, x1 - r.y)) << (16 * h);
-        }
-        const int at = n * kHd + (((lane >> 2) ^ (n & 7)) << 4) + (lane & 3) * 4;  // 128-byte swizzle
-        *reinterpret_cast<uint32_t*>(sq + at) = hi;
-        *reinterpret_cast<uint32_t*>(sq + N * kHd + at) = lo;
-        if (lane == 0) {
-          const int t = G == 1 ? g0 + n : __umulhi(g0 + n, inv_g), h = g0 + n - t * G;
-          b.unscale[n] = a.scale * kLog2e / up;
-          b.base[n] = 0.f;
-          b.lim[n] = n < it.rows ? min(it.key1, paged_key_limit(it.len, it.start + tok_base + t, a.causal_block)) : it.key1;
-          b.out[n] = (it.tok0 + tok_base + t) * a.hq + it.head * G + h;
-        }
-      }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&b.q_ready);
-      named_sync(2, 256);
-    }
+    if (threadIdx.x - 128 < N) b.base[threadIdx.x - 128] = 0.f;
+    paged_stage_queries<N, 8>(a, it, sq, sq + N * kHd, b.rows, threadIdx.x - 128, 2);
+    if (lane == 0) mbar_arrive(&b.q_ready);
+    named_sync(2, 256);
     // ---------------- softmax: a key a thread, half the columns a warpgroup ----------------
     constexpr int H = N / 2;
     const int q4 = warp & 3, key_lane = q4 * 32 + lane;  // TMEM lane
     const int col0 = warp < 8 ? 0 : H;
     const uint32_t lane_base = (static_cast<uint32_t>(q4 * 32) << 16) + col0;
     // keys from which some row's mask ends (rows are in token order, so the first has the least)
-    const int lim_min = b.lim[0];
+    const int lim_min = b.rows.lim[0];
     const bool mine = it.rows > col0;  // rows among this warpgroup's columns
     float sum[H];
 #pragma unroll
@@ -442,7 +388,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         if (it.key0 + (j + 1) * kKeys > lim_min) {
 #pragma unroll
           for (int n = 0; n < H; ++n)
-            if (key >= b.lim[col0 + n]) s[n] = -INFINITY;  // (also what a dead key's garbage gave)
+            if (key >= b.rows.lim[col0 + n]) s[n] = -INFINITY;  // (also what a dead key's garbage gave)
         }
 #pragma unroll
         for (int n = 0; n < H; n += 2) {
@@ -582,7 +528,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         if (it.splits == 1) {
 #pragma unroll
           for (int i = 0; i < 8; ++i)
-            if (n0 + i < it.rows) out[static_cast<size_t>(b.out[n0 + i]) * kHd] = __float2bfloat16_rn(x[i]);
+            if (n0 + i < it.rows) out[static_cast<size_t>(b.rows.out[n0 + i]) * kHd] = __float2bfloat16_rn(x[i]);
         } else {
 #pragma unroll
           for (int i = 0; i < 8; ++i)
@@ -608,42 +554,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     tc_fence_after_sync();
     tmem_dealloc(tmem, C::kCols);
   }
-  if (it.splits == 1) return;
-
-  // the tile's last item adds the partials, all threads: a row's weights 2^(base - max) / sum, then its columns
-  if (threadIdx.x == 0) b.last = atomicAdd(&a.arrived[it.tile], 1u) == static_cast<unsigned>(it.splits - 1);
-  __syncthreads();
-  if (!b.last) return;
-  __threadfence();
-  constexpr int kPart = N * kHd + 4 * N;  // floats
-  const float* first = reinterpret_cast<const float*>(a.part + it.part) - static_cast<size_t>(it.split) * kPart;
-  float* weight = reinterpret_cast<float*>(smem);  // [kMaxPagedSplits][N], over the K ring
-  for (int n = warp; n < it.rows; n += kThreads / 32) {  // a lane a split
-    float2 bs = make_float2(0.f, 0.f);
-    if (lane < it.splits) bs = __ldcg(reinterpret_cast<const float2*>(first + lane * kPart + N * kHd) + n);
-    float m = bs.y != 0.f ? bs.x : -INFINITY;
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-    const float f = bs.y != 0.f ? exp2f(bs.x - m) : 0.f;
-    float l = f * bs.y;
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
-    weight[lane * N + n] = l != 0.f ? f / l : 0.f;
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < it.rows * (kHd / 4); i += kThreads) {
-    const int n = i >> 5, c4 = i & 31;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-    for (int s = 0; s < it.splits; ++s) {
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(first + s * kPart + n * kHd) + c4);
-      const float f = weight[s * N + n];
-      acc.x += f * v.x, acc.y += f * v.y, acc.z += f * v.z, acc.w += f * v.w;
-    }
-    *reinterpret_cast<uint2*>(static_cast<bf16*>(a.out) + static_cast<size_t>(b.out[n]) * kHd + 4 * c4) =
-        make_uint2(pack_bf16x2(acc.x, acc.y), pack_bf16x2(acc.z, acc.w));
-  }
-  if (threadIdx.x == 0) a.arrived[it.tile] = 0;  // ready for the next call
+  if (it.splits > 1) paged_join<N, kThreads>(a, it, b.rows.out, smem);
 }
 
 template <int N>

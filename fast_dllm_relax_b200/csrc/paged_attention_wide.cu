@@ -92,7 +92,7 @@ struct Bars {
   uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
   uint64_t scale_full[4], q_ready, s_full[2], p_full[2], w_full[2], pv_done[2], o_final;
   uint32_t tmem;
-  int last;
+  PagedRows<kRows> rows;
   float4 scale[4][kKeys / 16];  // of tile j & 3, its 16-key groups: ks, log2 vs, 1 / vs
 };
 
@@ -117,7 +117,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       mbar_init(&b.pv_done[i], 1);
     }
     for (int i = 0; i < 4; ++i) mbar_init(&b.scale_full[i], 1);
-    mbar_init(&b.q_ready, 4);
+    mbar_init(&b.q_ready, 8);
     mbar_init(&b.o_final, 1);
     mbar_fence_init();
   }
@@ -132,8 +132,13 @@ __global__ void __launch_bounds__(kThreads, 2)
   pdl_trigger();
   pdl_wait();
   const PagedItem it = a.items[blockIdx.x];
-  const int G = a.hq / a.hkv;
   const int n_tiles = (it.key1 - it.key0 + kKeys - 1) / kKeys;
+
+  if (warp >= 4) {
+    paged_stage_queries<kRows, 8>(a, it, smem + kOffQ, smem + kOffQ + kQ, b.rows, threadIdx.x - 128, 2);
+    if (lane == 0) mbar_arrive(&b.q_ready);
+    named_sync(2, 256);
+  }
 
   if (warp < 4) set_registers<kRegsMisc, false>();
   if (warp == 0) {
@@ -290,50 +295,8 @@ __global__ void __launch_bounds__(kThreads, 2)
     const int q4 = warp & 3, tid = q4 * 32 + lane;
     const uint32_t lane_base = static_cast<uint32_t>(q4 * 32) << 16;
     const bool valid = tid < it.rows;
-    const int t = (it.row0 + (valid ? tid : 0)) / G, head = it.head * G + (it.row0 + (valid ? tid : 0)) % G;
-    const int lim = valid ? min(it.key1, paged_key_limit(it.len, it.start + t, a.causal_block)) : it.key0;
-    float unscale;
-    {  // the query row -> Qh, Ql with the 128-byte swizzle (zeros for padding rows)
-      const uint4* src = reinterpret_cast<const uint4*>(static_cast<const bf16*>(a.q) + static_cast<size_t>(it.tok0 + t) * a.ldq +
-                                                        static_cast<size_t>(head) * kHd);
-      uint4 v[16];
-#pragma unroll
-      for (int c = 0; c < 16; ++c) v[c] = valid ? src[c] : make_uint4(0u, 0u, 0u, 0u);
-      float m = 0.f;
-#pragma unroll
-      for (int c = 0; c < 16; ++c) {
-        const uint32_t w[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          m = fmaxf(m, fmaxf(fabsf(__uint_as_float(w[i] << 16)), fabsf(__uint_as_float(w[i] & 0xFFFF0000u))));
-      }
-      // exponent of m, kept where both the scale and its inverse are normal floats
-      const int e = min(max(static_cast<int>(__float_as_uint(m) >> 23) - 127, -110), 110);
-      const float up = m > 0.f ? __uint_as_float(static_cast<uint32_t>(127 + 7 - e) << 23) : 1.f;
-      unscale = a.scale * kLog2e / up;
-      uint8_t* dst = smem + kOffQ + tid * kHd;
-#pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        uint32_t hi[4], lo[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint4& u = v[2 * c + (i >> 1)];
-          const uint32_t w0 = i & 1 ? u.z : u.x, w1 = i & 1 ? u.w : u.y;
-          const float x0 = __uint_as_float(w0 << 16) * up, x1 = __uint_as_float(w0 & 0xFFFF0000u) * up;
-          const float x2 = __uint_as_float(w1 << 16) * up, x3 = __uint_as_float(w1 & 0xFFFF0000u) * up;
-          const uint16_t c0 = e4m3x2_from_f32(x0, x1), c1 = e4m3x2_from_f32(x2, x3);
-          const float2 r0 = f32x2_from_e4m3x2(c0), r1 = f32x2_from_e4m3x2(c1);
-          hi[i] = c0 | static_cast<uint32_t>(c1) << 16;
-          lo[i] = e4m3x2_from_f32(x0 - r0.x, x1 - r0.y) | static_cast<uint32_t>(e4m3x2_from_f32(x2 - r1.x, x3 - r1.y)) << 16;
-        }
-        *reinterpret_cast<uint4*>(dst + ((c ^ (tid & 7)) << 4)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        *reinterpret_cast<uint4*>(dst + kQ + ((c ^ (tid & 7)) << 4)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-      }
-    }
-    fence_proxy_async_smem();
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&b.q_ready);
-
+    const int lim = valid ? b.rows.lim[tid] : it.key0;
+    const float unscale = b.rows.unscale[tid];
     float base = 0.f, l = 0.f;
     bool ok = true, seated = false;  // seated: the base has been set (the row has attended a key)
     for (int j = 0; j < n_tiles; ++j) {
@@ -420,7 +383,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     tc_fence_after_sync();
     // a split tile leaves its partial: [128][128], then [128] (base, sum)
     const float inv = it.splits > 1 ? 1.f : l != 0.f ? 1.f / l : 0.f;
-    uint4* out = reinterpret_cast<uint4*>(static_cast<bf16*>(a.out) + (static_cast<size_t>(it.tok0 + t) * a.hq + head) * kHd);
+    uint4* out = reinterpret_cast<uint4*>(static_cast<bf16*>(a.out) + static_cast<size_t>(b.rows.out[tid]) * kHd);
     float4* part = a.part + it.part;
 #pragma unroll 1
     for (int c0 = 0; c0 < kHd; c0 += 32) {
@@ -458,51 +421,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     tc_fence_after_sync();
     tmem_dealloc(tmem, kTmemCols);
   }
-  if (it.splits == 1) return;
-
-  // the tile's last item adds the partials, all threads: a row's weights 2^(base - max) / sum, then its columns
-  if (threadIdx.x == 0) b.last = atomicAdd(&a.arrived[it.tile], 1u) == static_cast<unsigned>(it.splits - 1);
-  __syncthreads();
-  if (!b.last) return;
-  __threadfence();
-  constexpr int kPart = kRows * kHd + 4 * kRows;  // floats
-  const float* first = reinterpret_cast<const float*>(a.part + it.part) - static_cast<size_t>(it.split) * kPart;
-  float* weight = reinterpret_cast<float*>(smem);  // [kMaxPagedSplits][128], over the queries
-  if (threadIdx.x < it.rows) {
-    const int n = threadIdx.x;
-    float m = -INFINITY;
-#pragma unroll 8
-    for (int s = 0; s < it.splits; ++s) {
-      const float2 bs = __ldcg(reinterpret_cast<const float2*>(first + s * kPart + kRows * kHd) + n);
-      weight[s * kRows + n] = bs.x;
-      if (bs.y != 0.f) m = fmaxf(m, bs.x);
-    }
-    float l = 0.f;
-#pragma unroll 8
-    for (int s = 0; s < it.splits; ++s) {
-      const float2 bs = __ldcg(reinterpret_cast<const float2*>(first + s * kPart + kRows * kHd) + n);
-      const float f = bs.y != 0.f ? exp2f(bs.x - m) : 0.f;
-      weight[s * kRows + n] = f;
-      l += f * bs.y;
-    }
-    const float inv = l != 0.f ? 1.f / l : 0.f;
-    for (int s = 0; s < it.splits; ++s) weight[s * kRows + n] *= inv;
-  }
-  __syncthreads();
-#pragma unroll 2
-  for (int i = threadIdx.x; i < it.rows * (kHd / 4); i += kThreads) {
-    const int n = i >> 5, c4 = i & 31, row = it.row0 + n;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int s = 0; s < it.splits; ++s) {
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(first + s * kPart + n * kHd) + c4);
-      const float f = weight[s * kRows + n];
-      acc.x += f * v.x, acc.y += f * v.y, acc.z += f * v.z, acc.w += f * v.w;
-    }
-    bf16* dst = static_cast<bf16*>(a.out) + (static_cast<size_t>(it.tok0 + row / G) * a.hq + it.head * G + row % G) * kHd + 4 * c4;
-    *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(acc.x, acc.y), pack_bf16x2(acc.z, acc.w));
-  }
-  if (threadIdx.x == 0) a.arrived[it.tile] = 0;  // ready for the next call
+  if (it.splits > 1) paged_join<kRows, kThreads>(a, it, b.rows.out, smem);
 }
 
 // The register split only ever asks for what the launch brought: checked here, not by waiting for more.
