@@ -26,7 +26,7 @@ INCLUDE = PKG.parent / "include"
 
 SOURCES = ["gemm_tc.cu", "gemm_simt.cu", "attention.cu", "attention_tc.cu", "attention_tc_long.cu", "elementwise.cu",
            "paged.cu", "paged_append.cu", "paged_attention.cu", "paged_attention_narrow.cu",
-           "paged_attention_tc.cu", "paged_attention_wide.cu", "logprobs.cu", "model.cu", "decode.cu"]
+           "paged_attention_mma.cu", "logprobs.cu", "model.cu", "decode.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
          "--expt-relaxed-constexpr", "-DNDEBUG"]

@@ -417,8 +417,7 @@ int init_kernel_attributes() {
   if (e == cudaSuccess) e = static_cast<cudaError_t>(init_gemm_tc_attributes());
   if (e == cudaSuccess) e = static_cast<cudaError_t>(init_attention_tc_attributes());
   if (e == cudaSuccess) e = static_cast<cudaError_t>(init_paged_attention_attributes());
-  if (e == cudaSuccess) e = static_cast<cudaError_t>(init_paged_attention_tc_attributes());
-  if (e == cudaSuccess) e = static_cast<cudaError_t>(init_paged_attention_wide_attributes());
+  if (e == cudaSuccess) e = static_cast<cudaError_t>(init_paged_attention_mma_attributes());
   return e;
 }
 

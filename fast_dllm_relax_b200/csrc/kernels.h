@@ -199,8 +199,7 @@ int launch_attention(const AttnArgs& a, int max_q, int dtype, cudaStream_t s);
 int launch_attention_tc(const AttnArgs& a, const CUtensorMap* maps_dev, int max_q, int num_sms, cudaStream_t s);
 int init_attention_tc_attributes();
 int init_paged_attention_attributes();
-int init_paged_attention_tc_attributes();
-int init_paged_attention_wide_attributes();
+int init_paged_attention_mma_attributes();
 int init_kernel_attributes();  // opt-in shared memory sizes; once per device, before any capture
 
 int launch_embed(const int* ids, int n, const void* table, int vocab, int hidden, void* out, int dtype, int* err,

@@ -95,7 +95,7 @@ int plan_items(const fdllm_handle* h, const std::vector<PagedReq>& reqs, int cau
   const bool tc = c.head_dim == 128;
   const int unit = tc ? 16 : 8, narrow = tc ? 48 : 24;  // largest tile of the classes by rows
   auto is_wide = [&](long long rows) { return tc && rows > narrow; };
-  const long long slots = (tc ? 2LL : 3LL) * h->num_sms;
+  const long long slots = static_cast<long long>(tc ? 2 : kPagedNarrowCtas) * h->num_sms;
   auto tile_rows = [&](long long rows) {
     const int largest = is_wide(rows) ? 128 : narrow;
     const long long tiles = (rows + largest - 1) / largest;
@@ -276,14 +276,10 @@ int fdllm::paged_attention(fdllm_handle* h, const fdllm_paged_cache* cache, int 
   a.layer_row = static_cast<int>(codes / c.head_dim);
   a.part = h->paged_part.p;
   a.arrived = h->paged_ctr.p;
-  for (int k = 0; k < kPagedClasses; ++k) {
-    if (plan->priv[kPagedItems + k] == 0) continue;
-    a.items = reinterpret_cast<const PagedItem*>(plan_words + plan->priv[kPagedItemOff + k]);
-    const int n = plan->priv[kPagedItems + k];
-    CUDA_TRY(c.head_dim != 128  ? launch_paged_attention_narrow(a, k + 1, n, tm_k, tm_v, s)
-             : k == kPagedWide ? launch_paged_attention_wide(a, n, tm_k, tm_v, s)
-                               : launch_paged_attention_tc(a, 16 * (k + 1), n, tm_k, tm_v, s));
-  }
+  a.items = reinterpret_cast<const PagedItem*>(plan_words + plan->priv[kPagedItemOff]);
+  for (int k = kPagedClasses - 1, end = 0; k >= 0; --k) a.class_end[k] = end += plan->priv[kPagedItems + k];
+  CUDA_TRY(c.head_dim == 128 ? launch_paged_attention_mma(a, tm_k, tm_v, s)
+                             : launch_paged_attention_narrow(a, tm_k, tm_v, s));
   return FDLLM_OK;
 }
 
@@ -336,9 +332,9 @@ int fdllm_paged_plan_batch(fdllm_handle* h, const int32_t* rows, const int32_t* 
     if (h->dtype == FDLLM_BFLOAT16) FDLLM_TRY(plan_items(h, reqs, causal_block, &ip));
     out.priv[kPagedTiles] = ip.tiles;
     out.priv[kPagedParts] = static_cast<int>(ip.parts);
-    for (int c = 0; c < kPagedClasses; ++c) {
+    out.priv[kPagedItemOff] = at;
+    for (int c = kPagedClasses - 1; c >= 0; --c) {
       out.priv[kPagedItems + c] = static_cast<int>(ip.items[c].size());
-      out.priv[kPagedItemOff + c] = at;
       at += kPagedItemWords * static_cast<int>(ip.items[c].size());
     }
     out.words = at;
@@ -353,9 +349,11 @@ int fdllm_paged_plan_batch(fdllm_handle* h, const int32_t* rows, const int32_t* 
       std::memcpy(words + out.priv[kPagedPageOff], units.data(), units.size() * sizeof(PagedPageUnit));
     if (!q_units.empty())
       std::memcpy(words + out.priv[kPagedQOff], q_units.data(), q_units.size() * sizeof(PagedPageUnit));
-    for (int c = 0; c < kPagedClasses; ++c)
-      if (!ip.items[c].empty())
-        std::memcpy(words + out.priv[kPagedItemOff + c], ip.items[c].data(), ip.items[c].size() * sizeof(PagedItem));
+    int32_t* to = words + out.priv[kPagedItemOff];
+    for (int c = kPagedClasses - 1; c >= 0; --c) {
+      if (!ip.items[c].empty()) std::memcpy(to, ip.items[c].data(), ip.items[c].size() * sizeof(PagedItem));
+      to += kPagedItemWords * ip.items[c].size();
+    }
     return FDLLM_OK;
   });
 }

@@ -48,10 +48,11 @@ struct alignas(16) PagedItem {
 };
 static_assert(sizeof(PagedItem) == 4 * kPagedItemWords, "plan item layout");
 
-// Item classes, a launch each: tiles of 16, 32 and 48 query rows (keys on the MMA's M side) and of up to 128 (rows
+// Item classes, the largest tiles first in the plan: tiles of 16, 32 and 48 query rows (keys on the MMA's M side) and of up to 128 (rows
 // on it) at head_dim 128, of 8, 16 and 24 at the others (mma.sync).
 constexpr int kPagedClasses = 4;
 constexpr int kPagedWide = 3;
+constexpr int kPagedNarrowCtas = 3;  // CTAs on an SM at the other head sizes
 
 // fdllm_paged_plan::priv
 enum PagedPriv : int {
@@ -60,8 +61,8 @@ enum PagedPriv : int {
   kPagedTiles = 2,      // arrival counters needed
   kPagedParts = 3,      // workspace for partials, in 16-byte units
   kPagedItems = 4,      // [kPagedClasses] numbers of items
-  kPagedItemOff = kPagedItems + kPagedClasses,  // [kPagedClasses] word offsets of the items
-  kPagedQUnits = kPagedItemOff + kPagedClasses,  // number of query units
+  kPagedItemOff = kPagedItems + kPagedClasses,  // word offset of the items, class after class from the last
+  kPagedQUnits,         // number of query units
   kPagedQOff,           // word offset of the query units
   kPagedPrivEnd,
 };
@@ -100,6 +101,7 @@ struct PagedAttnArgs {
   float scale;
   void* out;
   const PagedItem* items;
+  int class_end[kPagedClasses];  // class c is the CTAs [class_end[c + 1], class_end[c])
   int layer_row;       // first row of this layer in the pool's maps (rows of head_dim codes)
   float4* part;        // partials of split tiles
   unsigned* arrived;   // [tiles] items done (zero between launches)
@@ -125,12 +127,9 @@ struct LogprobArgs {
 
 int launch_paged_append(const PagedAppendArgs& a, int dtype, cudaStream_t s);
 int launch_paged_attention_simt(const PagedAttnArgs& a, cudaStream_t s);  // fp32
-int launch_paged_attention_narrow(const PagedAttnArgs& a, int nt, int n_items, const CUtensorMap& k, const CUtensorMap& v,
-                                  cudaStream_t s);
-int launch_paged_attention_tc(const PagedAttnArgs& a, int cols, int n_items, const CUtensorMap& k, const CUtensorMap& v,
-                              cudaStream_t s);
-int launch_paged_attention_wide(const PagedAttnArgs& a, int n_items, const CUtensorMap& k, const CUtensorMap& v,
-                                cudaStream_t s);
+// bf16, all items in one launch (class_end[0] of them): head_dim 32 and 64; 128
+int launch_paged_attention_narrow(const PagedAttnArgs& a, const CUtensorMap& k, const CUtensorMap& v, cudaStream_t s);
+int launch_paged_attention_mma(const PagedAttnArgs& a, const CUtensorMap& k, const CUtensorMap& v, cudaStream_t s);
 // CTAs a row is split into, and chunks each.
 int logprobs_parts(int rows, int vocab, int dtype, int num_sms, int* part_chunks);
 int launch_logprobs(const LogprobArgs& a, int dtype, int parts, int part_chunks, cudaStream_t s);

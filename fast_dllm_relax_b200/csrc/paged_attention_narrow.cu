@@ -16,8 +16,7 @@
 //
 // Bound: HBM (one byte a cached value).  A producer warp keeps a ring of 64-key stages full with TMA copies
 // of whole pages (their rows of this KV head are contiguous), so the bytes in flight do not depend on the
-// compute warps' registers or progress; page ids and scales are read 32 pages at a time.  At head_dim 128
-// the copies are swizzled (128 bytes), which makes every fragment load free of bank conflicts: a thread of
+// compute warps' registers or progress; page ids and scales are read 32 pages at a time.  A thread of
 // the K fragment owns HD / 4 consecutive columns of rows g and g + 8, of the V fragment HD / 8 consecutive
 // columns of its four keys (the MMA's reduction and row orders are free as long as both operands agree).
 //
@@ -61,23 +60,18 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
 __device__ __forceinline__ uint32_t lo_pair(uint32_t w) { return f16x2_from_e4m3x2(static_cast<uint16_t>(w)); }
 __device__ __forceinline__ uint32_t hi_pair(uint32_t w) { return f16x2_from_e4m3x2(static_cast<uint16_t>(w >> 16)); }
 
-// N consecutive words of shared memory from byte offset `off` of row `row` of a tile of HD-byte rows, with
-// the 128-byte swizzle of a TMA copy (16-byte units xor row mod 8) at HD 128.
+// N consecutive words of shared memory from byte offset `off` of row `row` of a tile of HD-byte rows.
 template <int HD, int N>
 __device__ __forceinline__ void load_words(uint32_t* w, const uint8_t* tile, int row, int off) {
-#pragma unroll
-  for (int i = 0; i < N; i += 4) {
-    const int unit = off / 16 + i / 4;
-    const uint8_t* p = tile + row * HD + (HD == 128 ? (unit ^ (row & 7)) * 16 : off + 4 * i);
-    if constexpr (N >= 4) {
-      const uint4 u = *reinterpret_cast<const uint4*>(p);
-      w[i] = u.x, w[i + 1] = u.y, w[i + 2] = u.z, w[i + 3] = u.w;
-    } else if constexpr (N == 2) {
-      const uint2 u = *reinterpret_cast<const uint2*>(p);
-      w[0] = u.x, w[1] = u.y;
-    } else {
-      w[0] = *reinterpret_cast<const uint32_t*>(p);
-    }
+  const uint8_t* p = tile + row * HD + off;
+  if constexpr (N == 4) {
+    const uint4 u = *reinterpret_cast<const uint4*>(p);
+    w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
+  } else if constexpr (N == 2) {
+    const uint2 u = *reinterpret_cast<const uint2*>(p);
+    w[0] = u.x, w[1] = u.y;
+  } else {
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
   }
 }
 
@@ -93,9 +87,7 @@ struct Smem {
 };
 
 template <int HD, int NT>
-__global__ void __launch_bounds__(32 * (kWarps + 1))
-    paged_attn_narrow_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap tm_k,
-                             const __grid_constant__ CUtensorMap tm_v) {
+__device__ __forceinline__ void run(const PagedAttnArgs& a, const CUtensorMap& tm_k, const CUtensorMap& tm_v) {
   constexpr int R = 8 * NT, KS = HD / 16;  // query rows; MMA steps of a score, and of the head columns
   using S = Smem<HD, NT>;
   extern __shared__ uint8_t smem_raw[];
@@ -392,36 +384,31 @@ __global__ void __launch_bounds__(32 * (kWarps + 1))
   if (threadIdx.x == 0) a.arrived[it.tile] = 0;  // ready for the next call
 }
 
-template <int HD, int NT>
-int launch_nt(const PagedAttnArgs& a, int n_items, const CUtensorMap& k, const CUtensorMap& v, cudaStream_t s) {
-  return launch_k(paged_attn_narrow_kernel<HD, NT>, dim3(n_items), dim3(32 * (kWarps + 1)), Smem<HD, NT>::kBytes, s, a, k, v);
-}
+// One launch for all classes, each a range of the grid.
 template <int HD>
-int launch_hd(const PagedAttnArgs& a, int nt, int n, const CUtensorMap& k, const CUtensorMap& v, cudaStream_t s) {
-  return nt == 1 ? launch_nt<HD, 1>(a, n, k, v, s) : nt == 2 ? launch_nt<HD, 2>(a, n, k, v, s) : launch_nt<HD, 3>(a, n, k, v, s);
-}
-template <int HD, int NT>
-cudaError_t opt_in() {
-  return cudaFuncSetAttribute(paged_attn_narrow_kernel<HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                              Smem<HD, NT>::kBytes);
+__global__ void __launch_bounds__(32 * (kWarps + 1), kPagedNarrowCtas)
+    paged_attn_narrow_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap tm_k,
+                             const __grid_constant__ CUtensorMap tm_v) {
+  const int i = blockIdx.x;
+  if (i < a.class_end[2]) run<HD, 3>(a, tm_k, tm_v);
+  else if (i < a.class_end[1]) run<HD, 2>(a, tm_k, tm_v);
+  else run<HD, 1>(a, tm_k, tm_v);
 }
 
 }  // namespace
 
 int init_paged_attention_attributes() {
-  for (cudaError_t e : {opt_in<32, 1>(), opt_in<32, 2>(), opt_in<32, 3>(), opt_in<64, 1>(), opt_in<64, 2>(), opt_in<64, 3>(),
-                        opt_in<128, 1>(), opt_in<128, 2>(), opt_in<128, 3>()})
-    if (e != cudaSuccess) return e;
-  return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(paged_attn_narrow_kernel<32>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             Smem<32, 3>::kBytes);
+  return e != cudaSuccess ? e
+                          : cudaFuncSetAttribute(paged_attn_narrow_kernel<64>,
+                                                 cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<64, 3>::kBytes);
 }
 
-int launch_paged_attention_narrow(const PagedAttnArgs& a, int nt, int n_items, const CUtensorMap& k, const CUtensorMap& v,
-                                  cudaStream_t s) {
-  switch (a.hd) {
-    case 32: return launch_hd<32>(a, nt, n_items, k, v, s);
-    case 64: return launch_hd<64>(a, nt, n_items, k, v, s);
-    default: return launch_hd<128>(a, nt, n_items, k, v, s);
-  }
+int launch_paged_attention_narrow(const PagedAttnArgs& a, const CUtensorMap& k, const CUtensorMap& v, cudaStream_t s) {
+  const dim3 grid(a.class_end[0]), block(32 * (kWarps + 1));
+  return a.hd == 32 ? launch_k(paged_attn_narrow_kernel<32>, grid, block, Smem<32, 3>::kBytes, s, a, k, v)
+                    : launch_k(paged_attn_narrow_kernel<64>, grid, block, Smem<64, 3>::kBytes, s, a, k, v);
 }
 
 }  // namespace fdllm

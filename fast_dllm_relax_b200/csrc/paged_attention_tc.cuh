@@ -26,32 +26,21 @@
 //
 // A tile whose keys are split over several items joins them through the workspace as in
 // paged_attention_narrow.cu: the last item to arrive adds the partials in item order.
-#include "paged.h"
+#pragma once
+#include "paged_mma.cuh"
 
 namespace fdllm {
-
-namespace {
+namespace paged_tc {
 
 constexpr int kKeys = 128;
 constexpr int kHd = 128;
 constexpr int kTile = kKeys * kHd;  // bytes of a K or V tile
-constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kTrip = 8.f, kSeat = 3.f;
 
 // Instruction descriptor, kind::f8f6f4: fp32 accumulator, both operands e4m3, M 128; S = K Q^T has both K-major,
 // O^T = V^T P^T both MN-major.
 constexpr uint32_t idesc_s(int n) { return (1u << 4) | (static_cast<uint32_t>(n >> 3) << 17) | ((128u >> 4) << 24); }
 constexpr uint32_t idesc_o(int n) { return idesc_s(n) | (1u << 15) | (1u << 16); }
-
-// D[tmem] (+)= A[smem] * B[smem]^T, e4m3 operands, fp32 accumulate, one CTA.
-__device__ __forceinline__ void mma_f8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
 
 // Shared-memory descriptor of an unswizzled MN-major operand: core matrices of 8 K rows by 16 MN bytes
 // (128 B, row after row), `mn` bytes between core matrices along MN and `k` along K.
@@ -81,11 +70,6 @@ __device__ __forceinline__ void after_wait(uint32_t (&r)[8]) {
   for (int i = 0; i < 8; ++i) asm volatile("" : "+r"(r[i]));
 }
 
-__device__ __forceinline__ float exp2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 __device__ __forceinline__ uint16_t e4m3x2_from_f16x2(__half2 h) {
   uint16_t r;
   asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(r) : "r"(*reinterpret_cast<const uint32_t*>(&h)));
@@ -131,8 +115,7 @@ __device__ __forceinline__ float reduce_columns(const float* x, int lane, F f) {
   return f(v[0], __shfl_xor_sync(0xffffffffu, v[0], 16));
 }
 
-constexpr int kThreads = 384;
-constexpr int kRegsLaunch = 80, kRegsMisc = 48, kRegsSoftmax = 96;
+constexpr int kRegsMisc = 48, kRegsSoftmax = 96;
 static_assert(kRegsMisc + 2 * kRegsSoftmax == 3 * kRegsLaunch, "the split is the launch's registers");
 
 template <int N>
@@ -165,24 +148,13 @@ template <int N>
 constexpr bool two_ctas() { return Cfg<N>::kBytes + static_cast<int>(sizeof(Bars<N>)) + 1024 <= 228 * 1024 / 2; }
 static_assert(two_ctas<16>() && two_ctas<32>() && two_ctas<48>(), "two CTAs per SM, with the system's 1 KB each");
 
-template <int kRegs, bool kGrow>
-__device__ __forceinline__ void set_registers() {
-  if constexpr (kGrow) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs));
-  else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs));
-}
-
-}  // namespace
-
+// One item: `smem` 1024-byte aligned, `b` in static shared memory.
 template <int N>
-__global__ void __launch_bounds__(kThreads, 2)
-    paged_attn_tc_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap tm_k,
-                         const __grid_constant__ CUtensorMap tm_v) {
+__device__ __forceinline__ void run(const PagedAttnArgs& a, const CUtensorMap& tm_k, const CUtensorMap& tm_v, uint8_t* smem,
+                                    Bars<N>& b) {
   using C = Cfg<N>;
   constexpr int kStages = C::kStages;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sq = smem + C::kOffQ;
-  __shared__ Bars<N> b;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
@@ -557,34 +529,5 @@ __global__ void __launch_bounds__(kThreads, 2)
   if (it.splits > 1) paged_join<N, kThreads>(a, it, b.rows.out, smem);
 }
 
-template <int N>
-static int launch_n(const PagedAttnArgs& a, int n_items, const CUtensorMap& k, const CUtensorMap& v, cudaStream_t s) {
-  return launch_k(paged_attn_tc_kernel<N>, dim3(n_items), dim3(kThreads), Cfg<N>::kBytes, s, a, k, v);
-}
-// The register split only ever asks for what the launch brought: checked here, not by waiting for more.
-template <int N>
-static cudaError_t opt_in() {
-  cudaFuncAttributes f;
-  cudaError_t e = cudaFuncGetAttributes(&f, paged_attn_tc_kernel<N>);
-  if (e == cudaSuccess && f.numRegs < kRegsLaunch) e = cudaErrorInvalidKernelImage;
-  return e != cudaSuccess ? e
-                          : cudaFuncSetAttribute(paged_attn_tc_kernel<N>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                 Cfg<N>::kBytes);
-}
-
-int init_paged_attention_tc_attributes() {
-  for (cudaError_t e : {opt_in<16>(), opt_in<32>(), opt_in<48>()})
-    if (e != cudaSuccess) return e;
-  return cudaSuccess;
-}
-
-int launch_paged_attention_tc(const PagedAttnArgs& a, int cols, int n_items, const CUtensorMap& k, const CUtensorMap& v,
-                              cudaStream_t s) {
-  switch (cols) {
-    case 16: return launch_n<16>(a, n_items, k, v, s);
-    case 32: return launch_n<32>(a, n_items, k, v, s);
-    default: return launch_n<48>(a, n_items, k, v, s);
-  }
-}
-
+}  // namespace paged_tc
 }  // namespace fdllm

@@ -25,11 +25,11 @@
 //
 // A tile whose keys are split over several items joins them through the workspace as in
 // paged_attention_narrow.cu: the last item to arrive adds the partials in item order.
-#include "paged.h"
+#pragma once
+#include "paged_mma.cuh"
 
 namespace fdllm {
-
-namespace {
+namespace paged_wide {
 
 constexpr int kRows = 128, kKeys = 64, kHd = 128;
 constexpr int kTile = kKeys * kHd;      // bytes of a K or V tile as cached
@@ -38,10 +38,8 @@ constexpr int kV16 = kKeys * kHd * 2;   // bytes of a widened V tile: two sub-ti
 constexpr int kOffQ = 0, kOffK = 2 * kQ, kOffV = kOffK + 2 * kTile, kOffV16 = kOffV + 2 * kTile;
 constexpr int kBytes = 1024 + kOffV16 + 2 * kV16;
 constexpr uint32_t kTmemS = 0, kTmemO = 128, kTmemCols = 256;  // S: two buffers of 64 columns
-constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kTrip = 15.f, kSeat = 8.f;
-constexpr int kThreads = 384;
-constexpr int kRegsLaunch = 80, kRegsMisc = 48, kRegsSoftmax = 144, kRegsWiden = 48;
+constexpr int kRegsMisc = 48, kRegsSoftmax = 144, kRegsWiden = 48;
 static_assert(kRegsMisc + kRegsSoftmax + kRegsWiden == 3 * kRegsLaunch, "the split is the launch's registers");
 static_assert(2 * (kBytes + 2048) <= 228 * 1024, "two CTAs per SM");
 
@@ -50,14 +48,6 @@ static_assert(2 * (kBytes + 2048) <= 228 * 1024, "two CTAs per SM");
 constexpr uint32_t kIdescS = (1u << 4) | ((kKeys >> 3) << 17) | ((128u >> 4) << 24);
 constexpr uint32_t kIdescO = (1u << 4) | (1u << 16) | ((kHd >> 3) << 17) | ((128u >> 4) << 24);
 
-__device__ __forceinline__ void mma_f8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
 // D[tmem] (+)= A[tmem] * B[smem]^T, f16 operands (two to a TMEM column of A).
 __device__ __forceinline__ void mma_f16_ta(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -72,20 +62,9 @@ __device__ __forceinline__ void after_wait(uint32_t (&r)[32]) {  // a load's reg
 #pragma unroll
   for (int i = 0; i < 32; ++i) asm volatile("" : "+r"(r[i]));
 }
-__device__ __forceinline__ float exp2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
-}
-
-template <int kRegs, bool kGrow>
-__device__ __forceinline__ void set_registers() {
-  if constexpr (kGrow) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs));
-  else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs));
 }
 
 struct Bars {
@@ -96,14 +75,9 @@ struct Bars {
   float4 scale[4][kKeys / 16];  // of tile j & 3, its 16-key groups: ks, log2 vs, 1 / vs
 };
 
-}  // namespace
-
-__global__ void __launch_bounds__(kThreads, 2)
-    paged_attn_wide_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap tm_k,
-                           const __grid_constant__ CUtensorMap tm_v) {
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ Bars b;
+// One item: `smem` 1024-byte aligned, `b` in static shared memory.
+__device__ __forceinline__ void run(const PagedAttnArgs& a, const CUtensorMap& tm_k, const CUtensorMap& tm_v, uint8_t* smem,
+                                    Bars& b) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
@@ -424,17 +398,5 @@ __global__ void __launch_bounds__(kThreads, 2)
   if (it.splits > 1) paged_join<kRows, kThreads>(a, it, b.rows.out, smem);
 }
 
-// The register split only ever asks for what the launch brought: checked here, not by waiting for more.
-int init_paged_attention_wide_attributes() {
-  cudaFuncAttributes f;
-  cudaError_t e = cudaFuncGetAttributes(&f, paged_attn_wide_kernel);
-  if (e == cudaSuccess && f.numRegs < kRegsLaunch) e = cudaErrorInvalidKernelImage;
-  return e != cudaSuccess ? e : cudaFuncSetAttribute(paged_attn_wide_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
-}
-
-int launch_paged_attention_wide(const PagedAttnArgs& a, int n_items, const CUtensorMap& k, const CUtensorMap& v,
-                                cudaStream_t s) {
-  return launch_k(paged_attn_wide_kernel, dim3(n_items), dim3(kThreads), kBytes, s, a, k, v);
-}
-
+}  // namespace paged_wide
 }  // namespace fdllm

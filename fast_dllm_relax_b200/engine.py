@@ -301,6 +301,10 @@ class Engine:
         if (vocab > 1 and one != 1) or (n > 1 and ld < vocab):
             x = x.contiguous()
             ld = vocab
+        top = int(top)
+        ent = torch.empty(n, dtype=torch.float32, device=self.device)
+        tlp = torch.empty((n, max(top, 0)), dtype=torch.float32, device=self.device)
+        ids = torch.empty_like(tlp, dtype=torch.int32)
         tg = lp = None
         if targets is not None:
             tg = targets
@@ -308,11 +312,7 @@ class Engine:
                 tg = tg.to(self.device, torch.int32).contiguous().reshape(-1)
             if tg.numel() != n:
                 raise ValueError("logprobs: one target per row")
-            lp = torch.empty(n, dtype=torch.float32, device=self.device)
-        ent = torch.empty(n, dtype=torch.float32, device=self.device)
-        top = int(top)
-        ids = torch.empty((n, max(top, 0)), dtype=torch.int32, device=self.device)
-        tlp = torch.empty((n, max(top, 0)), dtype=torch.float32, device=self.device)
+            lp = torch.empty_like(ent)
         _lib.check(self.lib.fdllm_logprobs(self._h, x.data_ptr(), code, n, vocab, ld if n > 1 else vocab, _ptr(tg), top,
                                            _ptr(lp), ent.data_ptr(), ids.data_ptr() if top > 0 else None,
                                            tlp.data_ptr() if top > 0 else None, self._raw_stream()))
@@ -360,7 +360,7 @@ class Engine:
         out = None
         if q is not None:
             q = self._token_rows(q, rows, q_cols, "paged_append: q")
-            out = torch.empty((rows, q_cols), dtype=self.dtype, device=self.device)
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
         cos = sin = None
         positions = 0
         if rope is not None:
@@ -383,9 +383,8 @@ class Engine:
         [total_rows, heads * head_dim], rotated -> [total_rows, heads * head_dim].  scale defaults to
         head_dim ** -0.5."""
         self._paged(cache, plan, table, "paged_attention")
-        rows = plan.total_rows
-        q = self._token_rows(q, rows, self._q_cols, "paged_attention: q")
-        out = torch.empty((rows, self._q_cols), dtype=self.dtype, device=self.device)
+        q = self._token_rows(q, plan.total_rows, self._q_cols, "paged_attention: q")
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
         _lib.check(self.lib.fdllm_paged_attention(
             self._h, cache.ref, layer, plan.ref, plan.words_ptr, table.data_ptr(), table.shape[1], q.data_ptr(),
             q.stride(0), self.cfg.head_dim ** -0.5 if scale is None else scale, out.data_ptr(), self._raw_stream()))
