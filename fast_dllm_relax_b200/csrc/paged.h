@@ -253,107 +253,108 @@ __device__ __forceinline__ void paged_stage_queries(const PagedAttnArgs& a, cons
   __syncwarp();
 }
 
-// The columns of paged_join: RB rows of a warp by SU splits in flight.
-template <int PR, int THREADS, int RB, int SU>
+// The columns of paged_join: rows n0, n0 + step, .. (RB of them) of a warp, SU partials in flight.
+template <int PR, int RB, int SU>
 __device__ __forceinline__ void paged_join_rows(const PagedAttnArgs& a, const PagedItem& it, const float* first,
-                                                const float* weight, const int* out_row) {
-  constexpr int kPart = PR * 128 + 4 * PR, kWarpsJ = THREADS / 32;
+                                                const float* weight, const int* out_row, int n0, int step) {
+  constexpr int kPart = PR * 132;  // floats
   const int lane = threadIdx.x & 31;
-#pragma unroll 1
-  for (int n0 = threadIdx.x >> 5; n0 < it.rows; n0 += kWarpsJ * RB) {
-    float4 acc[RB];
+  float4 acc[RB];
 #pragma unroll
-    for (int j = 0; j < RB; ++j) acc[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 1
-    for (int s0 = 0; s0 < it.splits; s0 += SU) {
-      float4 v[RB][SU];
-#pragma unroll
-      for (int j = 0; j < RB; ++j)
-#pragma unroll
-        for (int u = 0; u < SU; ++u) {
-          const int n = n0 + j * kWarpsJ, s = s0 + u;
-          if (n < it.rows && s < it.splits) v[j][u] = __ldcg(reinterpret_cast<const float4*>(first + s * kPart + n * 128) + lane);
-        }
-#pragma unroll
-      for (int j = 0; j < RB; ++j)
-#pragma unroll
-        for (int u = 0; u < SU; ++u) {
-          const int n = n0 + j * kWarpsJ, s = s0 + u;
-          if (n < it.rows && s < it.splits) {
-            const float f = weight[s * PR + n];
-            const float4 x = v[j][u];
-            acc[j].x += f * x.x, acc[j].y += f * x.y, acc[j].z += f * x.z, acc[j].w += f * x.w;
-          }
-        }
-    }
+  for (int j = 0; j < RB; ++j) acc[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+  const float4* from = reinterpret_cast<const float4*>(first + n0 * 128) + lane;
+  const float* w = weight + n0;
+#pragma unroll SU
+  for (int s = 0; s < it.splits; ++s, from += kPart / 4, w += PR) {
 #pragma unroll
     for (int j = 0; j < RB; ++j) {
-      const int n = n0 + j * kWarpsJ;
-      if (n < it.rows)
-        *reinterpret_cast<uint2*>(static_cast<bf16*>(a.out) + static_cast<size_t>(out_row[n]) * 128 + 4 * lane) =
-            make_uint2(pack_bf16x2(acc[j].x, acc[j].y), pack_bf16x2(acc[j].z, acc[j].w));
+      const float4 x = __ldcg(from + j * step * 32);
+      const float f = w[j * step];
+      acc[j].x += f * x.x, acc[j].y += f * x.y, acc[j].z += f * x.z, acc[j].w += f * x.w;
     }
   }
+#pragma unroll
+  for (int j = 0; j < RB; ++j)
+    *reinterpret_cast<uint2*>(static_cast<bf16*>(a.out) + static_cast<size_t>(out_row[n0 + j * step]) * 128 + 4 * lane) =
+        make_uint2(pack_bf16x2(acc[j].x, acc[j].y), pack_bf16x2(acc[j].z, acc[j].w));
 }
 
 // The last item of a split tile to arrive (a.arrived) adds the tile's partials in item order, all THREADS threads:
-// out = sum_s w_s O_s / sum_s w_s l_s, w_s = 2^(base_s - max base).  An item leaves [PR][128] columns of O, then
-// PR pairs (base, sum).  `scratch`: 16 bytes and 4 PR a split of shared memory that nothing else uses any more.  Every thread calls it,
-// after a __threadfence() by those that wrote the item's partial; the counter is zero again afterwards.
+// out = sum_s w_s O_s / sum_s w_s l_s, w_s = 2^(base_s - max base).  An item leaves [PR][128] columns of O, then PR
+// pairs (base, sum).  Bound by what one SM reads from L2, about 42 bytes a clock: 12000 clocks for 64 rows x 15
+// partials, 3000 for 128 x 2.  `scratch`: 16 bytes and 8 PR a split of shared memory that nothing else uses any more.
+// Every thread calls it; the counter is zero again afterwards.
 template <int PR, int THREADS>
 __device__ __forceinline__ void paged_join(const PagedAttnArgs& a, const PagedItem& it, const int* out_row, uint8_t* scratch) {
-  constexpr int kPart = PR * 128 + 4 * PR;  // floats
+  constexpr int kPart = PR * 132, kWarpsJ = THREADS / 32;
   int* last = reinterpret_cast<int*>(scratch);
+  float* weight = reinterpret_cast<float*>(last + 4);  // [splits][PR]
   __syncthreads();
-  if (threadIdx.x == 0) *last = atomicAdd(&a.arrived[it.tile], 1u) == static_cast<unsigned>(it.splits - 1);
+  if (threadIdx.x == 0) {  // the barriers carry its fences to the other threads
+    __threadfence();
+    *last = atomicAdd(&a.arrived[it.tile], 1u) == static_cast<unsigned>(it.splits - 1);
+    __threadfence();
+  }
   __syncthreads();
   if (!*last) return;
-  __threadfence();
   const float* first = reinterpret_cast<const float*>(a.part + it.part) - static_cast<size_t>(it.split) * kPart;
-  float* weight = reinterpret_cast<float*>(last + 4);  // [splits][PR]
-  const int lane = threadIdx.x & 31;
-  // The weights.  Many rows: a thread a row, its splits one after the other.  No more rows than warps: a warp a row,
-  // a lane a split.  (Tiles of 128 rows, 8 requests of 100 tokens: 28.9 us a call instead of 33.5 with a warp a row; 6 rows by 32
-  // splits: 17.8 instead of 28.4 with a thread a row.)
-  if (it.rows > THREADS / 32) {
-    if (threadIdx.x < PR) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  // The weights.  Many rows: every thread loads pairs, then a thread a row; no more rows than warps: a warp a row, a
+  // lane a partial.
+  if (it.rows > kWarpsJ) {
+    float* sum = weight + it.splits * PR;
+    const int n_pairs = it.splits * PR;
+#pragma unroll 1
+    for (int i0 = threadIdx.x; i0 < n_pairs; i0 += 4 * THREADS) {
+      float2 p[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int i = i0 + j * THREADS, s = i / PR, n = i - s * PR;
+        p[j] = make_float2(0.f, 0.f);
+        if (i < n_pairs && n < it.rows) p[j] = __ldcg(reinterpret_cast<const float2*>(first + s * kPart + PR * 128) + n);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (i0 + j * THREADS < n_pairs)
+          weight[i0 + j * THREADS] = p[j].y != 0.f ? p[j].x : -INFINITY, sum[i0 + j * THREADS] = p[j].y;
+    }
+    __syncthreads();
+    if (threadIdx.x < it.rows) {
       const int n = threadIdx.x;
       float m = -INFINITY, l = 0.f;
 #pragma unroll 4
-      for (int s = 0; s < it.splits; ++s) {
-        const float2 p = __ldcg(reinterpret_cast<const float2*>(first + s * kPart + PR * 128) + n);
-        weight[s * PR + n] = p.y != 0.f ? p.x : -INFINITY;
-        m = fmaxf(m, weight[s * PR + n]);
-      }
+      for (int s = 0; s < it.splits; ++s) m = fmaxf(m, weight[s * PR + n]);
 #pragma unroll 4
       for (int s = 0; s < it.splits; ++s) {
         const float f = m != -INFINITY ? exp2f(weight[s * PR + n] - m) : 0.f;
         weight[s * PR + n] = f;
-        l += f * __ldcg(first + s * kPart + PR * 128 + 2 * n + 1);
+        l += f * sum[s * PR + n];
       }
       const float inv = l != 0.f ? 1.f / l : 0.f;
 #pragma unroll 4
       for (int s = 0; s < it.splits; ++s) weight[s * PR + n] *= inv;
     }
-  } else {
+    __syncthreads();
+    int n = warp;
 #pragma unroll 1
-    for (int n = threadIdx.x >> 5; n < it.rows; n += THREADS / 32) {
-      float2 bs = make_float2(0.f, 0.f);
-      if (lane < it.splits) bs = __ldcg(reinterpret_cast<const float2*>(first + lane * kPart + PR * 128) + n);
-      float m = bs.y != 0.f ? bs.x : -INFINITY;
+    for (; n + 3 * kWarpsJ < it.rows; n += 4 * kWarpsJ)
+      paged_join_rows<PR, 4, 2>(a, it, first, weight, out_row, n, kWarpsJ);
+#pragma unroll 1
+    for (; n < it.rows; n += kWarpsJ) paged_join_rows<PR, 1, 8>(a, it, first, weight, out_row, n, kWarpsJ);
+  } else if (warp < it.rows) {
+    float2 bs = make_float2(0.f, 0.f);
+    if (lane < it.splits) bs = __ldcg(reinterpret_cast<const float2*>(first + lane * kPart + PR * 128) + warp);
+    float m = bs.y != 0.f ? bs.x : -INFINITY;
 #pragma unroll
-      for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-      const float f = bs.y != 0.f ? exp2f(bs.x - m) : 0.f;
-      float l = f * bs.y;
+    for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+    const float f = bs.y != 0.f ? exp2f(bs.x - m) : 0.f;
+    float l = f * bs.y;
 #pragma unroll
-      for (int d = 16; d > 0; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
-      if (lane < it.splits) weight[lane * PR + n] = l != 0.f ? f / l : 0.f;
-    }
+    for (int d = 16; d > 0; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+    if (lane < it.splits) weight[lane * PR + warp] = l != 0.f ? f / l : 0.f;
+    __syncwarp();
+    paged_join_rows<PR, 1, 8>(a, it, first, weight, out_row, warp, kWarpsJ);
   }
-  __syncthreads();
-  // a warp a row, four columns a lane; eight loads in flight, over splits where there are few rows
-  if (it.rows <= THREADS / 32) paged_join_rows<PR, THREADS, 1, 8>(a, it, first, weight, out_row);
-  else paged_join_rows<PR, THREADS, 4, 2>(a, it, first, weight, out_row);
   if (threadIdx.x == 0) a.arrived[it.tile] = 0;  // ready for the next call
 }
 #endif

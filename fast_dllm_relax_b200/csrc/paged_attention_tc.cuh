@@ -511,7 +511,6 @@ __device__ __forceinline__ void run(const PagedAttnArgs& a, const CUtensorMap& t
     if (it.splits > 1) {
       if (t < it.rows)
         reinterpret_cast<float2*>(reinterpret_cast<float*>(a.part + it.part) + N * kHd)[t] = make_float2(b.base[t], b.delta[t]);
-      __threadfence();
     }
     tc_fence_before_sync();
   }

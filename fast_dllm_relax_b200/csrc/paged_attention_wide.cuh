@@ -380,7 +380,6 @@ __device__ __forceinline__ void run(const PagedAttnArgs& a, const CUtensorMap& t
     }
     if (it.splits > 1) {
       if (valid) reinterpret_cast<float2*>(part + kRows * (kHd / 4))[tid] = make_float2(base, l);
-      __threadfence();
     }
     tc_fence_before_sync();
   }
