@@ -190,12 +190,12 @@ struct PagedRows {
   int lim[PR];        // cache rows it attends within the item's range (padding rows: the range's end)
 };
 
-// The query rows of an item as two e4m3 terms Qh + Ql (128-byte rows with the 128-byte swizzle, zeros for padding
-// rows), by WARPS warps from thread `tid` on (named barrier `bar`): a warp a row, four columns a lane.  A row is
-// scaled by the power of two that puts its largest element into [2^7, 2^8).  Four rows go through their chain of
-// dependent steps together while the next four are loaded; the loop over them is rolled, since code that runs once
-// is fetched cold.
-template <int PR, int WARPS>
+// The query rows of an item as two e4m3 terms Qh + Ql (128-byte rows with the 128-byte swizzle), by WARPS warps from
+// thread `tid` on (named barrier `bar`): a warp a row, four columns a lane.  kPad: padding rows get zeros, else only
+// those up to a multiple of 4 WARPS are written.  A row is scaled by the power of two that puts its largest element
+// into [2^7, 2^8).  Four rows go through their chain of dependent steps together while the next four are loaded; the
+// loop over them is rolled, since code that runs once is fetched cold.
+template <int PR, int WARPS, bool kPad>
 __device__ __forceinline__ void paged_stage_queries(const PagedAttnArgs& a, const PagedItem& it, uint8_t* qh, uint8_t* ql,
                                                     PagedRows<PR>& rows, int tid, int bar) {
   constexpr float kLog2e = 1.4426950408889634f;
@@ -215,7 +215,7 @@ __device__ __forceinline__ void paged_stage_queries(const PagedAttnArgs& a, cons
 #pragma unroll
   for (int i = 0; i < 4; ++i) next[i] = load(w + i * WARPS);
 #pragma unroll 1
-  for (int n0 = w; n0 < PR; n0 += 4 * WARPS) {
+  for (int n0 = w; n0 < (kPad ? PR : it.rows); n0 += 4 * WARPS) {
     uint2 u[4];
     float m[4];
 #pragma unroll

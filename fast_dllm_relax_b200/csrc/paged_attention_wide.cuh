@@ -109,7 +109,7 @@ __device__ __forceinline__ void run(const PagedAttnArgs& a, const CUtensorMap& t
   const int n_tiles = (it.key1 - it.key0 + kKeys - 1) / kKeys;
 
   if (warp >= 4) {
-    paged_stage_queries<kRows, 8>(a, it, smem + kOffQ, smem + kOffQ + kQ, b.rows, threadIdx.x - 128, 2);
+    paged_stage_queries<kRows, 8, false>(a, it, smem + kOffQ, smem + kOffQ + kQ, b.rows, threadIdx.x - 128, 2);
     if (lane == 0) mbar_arrive(&b.q_ready);
     named_sync(2, 256);
   }
@@ -277,6 +277,10 @@ __device__ __forceinline__ void run(const PagedAttnArgs& a, const CUtensorMap& t
       const int sb = j & 1, key0 = it.key0 + j * kKeys;
       ok = __all_sync(0xffffffffu, mbar_wait(&b.scale_full[j & 3], (j >> 2) & 1u) && mbar_wait(&b.s_full[sb], (j >> 1) & 1u));
       if (!ok) break;
+      if (q4 * 32 >= it.rows) {  // only padding rows: whatever P holds there stays in their rows of O
+        if (lane == 0) mbar_arrive(&b.p_full[sb]);
+        continue;
+      }
       tc_fence_after_sync();
       const uint32_t s_at = tmem + lane_base + kTmemS + sb * kKeys;
       float x[kKeys];
