@@ -181,72 +181,67 @@ __device__ __forceinline__ int paged_key_limit(int len, int pos, int causal_bloc
   return lim < len ? static_cast<int>(lim) : len;
 }
 
-// What the rows of an item need, one thread a row (integer divisions and all).
+// What the rows of an item need.
 template <int PR>
 struct PagedRows {
-  long long q[PR];    // element offset of the query row
   float unscale[PR];  // scale log2(e) over the power of two that the staged query is multiplied by
   int out[PR];        // (token, head) row of the output
   int lim[PR];        // cache rows it attends within the item's range (padding rows: the range's end)
 };
 
-// The query rows of an item as two e4m3 terms Qh + Ql (128-byte rows with the 128-byte swizzle), by WARPS warps from
-// thread `tid` on (named barrier `bar`): a warp a row, four columns a lane.  kPad: padding rows get zeros, else only
-// those up to a multiple of 4 WARPS are written.  A row is scaled by the power of two that puts its largest element
-// into [2^7, 2^8).  Four rows go through their chain of dependent steps together while the next four are loaded; the
-// loop over them is rolled, since code that runs once is fetched cold.
-template <int PR, int WARPS, bool kPad>
+// The query rows of an item as two e4m3 terms Qh + Ql (128-byte rows with the 128-byte swizzle), by 256 threads: 2 to 16
+// a row, as many as fit, each with consecutive columns.  kPad: padding rows get zeros, else they are left as they are.
+// A row is scaled by the power of two that puts its largest element into [2^7, 2^8).  (A warp a row, one column group a
+// lane, took twice the time at 128 rows: its five shuffles and its row's bookkeeping came once a row and warp.)
+template <int PR, bool kPad>
 __device__ __forceinline__ void paged_stage_queries(const PagedAttnArgs& a, const PagedItem& it, uint8_t* qh, uint8_t* ql,
-                                                    PagedRows<PR>& rows, int tid, int bar) {
+                                                    PagedRows<PR>& rows, int tid) {
   constexpr float kLog2e = 1.4426950408889634f;
-  const int lane = tid & 31, w = tid >> 5, G = a.hq / a.hkv;
-  if (tid < PR) {
-    const int row = it.row0 + min(tid, it.rows - 1), t = row / G, h = it.head * G + row - t * G;
-    rows.q[tid] = static_cast<long long>(it.tok0 + t) * a.ldq + static_cast<long long>(h) * 128;
-    rows.out[tid] = (it.tok0 + t) * a.hq + h;
-    rows.lim[tid] = tid < it.rows ? min(it.key1, paged_key_limit(it.len, it.start + t, a.causal_block)) : it.key1;
-  }
-  named_sync(bar, 32 * WARPS);
-  const bf16* q = static_cast<const bf16*>(a.q) + 4 * lane;
-  auto load = [&](int n) {
-    return n < it.rows ? *reinterpret_cast<const uint2*>(q + rows.q[n]) : make_uint2(0u, 0u);
-  };
-  uint2 next[4];
+  constexpr int kLanes = PR <= 16 ? 16 : PR <= 32 ? 8 : PR <= 48 ? 4 : 2, U = 16 / kLanes;  // threads a row, 16-byte loads
+  static_assert(PR * kLanes <= 256 && (PR * kLanes) % 32 == 0, "whole warps");
+  const int n = tid / kLanes, part = tid % kLanes, G = a.hq / a.hkv;
+  if (n < PR) {
+    const int row = it.row0 + min(n, it.rows - 1), t = row / G, h = it.head * G + row - t * G;
+    const uint4* src = reinterpret_cast<const uint4*>(static_cast<const bf16*>(a.q) + static_cast<long long>(it.tok0 + t) * a.ldq +
+                                                      static_cast<long long>(h) * 128) + part * U;
+    uint4 u[U];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) next[i] = load(w + i * WARPS);
-#pragma unroll 1
-  for (int n0 = w; n0 < (kPad ? PR : it.rows); n0 += 4 * WARPS) {
-    uint2 u[4];
-    float m[4];
+    for (int i = 0; i < U; ++i) u[i] = n < it.rows ? __ldg(src + i) : make_uint4(0u, 0u, 0u, 0u);
+    uint32_t m2 = 0u;  // the largest magnitudes of the even and the odd columns
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      u[i] = next[i];
-      next[i] = load(n0 + (4 + i) * WARPS);
-      m[i] = __uint_as_float(max(max((u[i].x & 0x7FFFu) << 16, u[i].x & 0x7FFF0000u),  // the largest magnitude
-                                 max((u[i].y & 0x7FFFu) << 16, u[i].y & 0x7FFF0000u)));
-    }
+    for (int i = 0; i < U; ++i)
+      m2 = __vmaxu2(__vmaxu2(m2, __vmaxu2(u[i].x & 0x7FFF7FFFu, u[i].y & 0x7FFF7FFFu)),
+                    __vmaxu2(u[i].z & 0x7FFF7FFFu, u[i].w & 0x7FFF7FFFu));
+    uint32_t m = max(m2 & 0xFFFFu, m2 >> 16);
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1)
+    for (int d = kLanes / 2; d > 0; d >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
+    // exponent of the maximum (a bf16's bits), kept where both the scale and its inverse are normal floats
+    int e = min(max(static_cast<int>(m >> 7) - 127, -110), 110);
+    if (m == 0u) e = 7;
+    const float up = __uint_as_float(static_cast<uint32_t>(127 + 7 - e) << 23);
+    if (kPad || n < it.rows) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) m[i] = fmaxf(m[i], __shfl_xor_sync(0xffffffffu, m[i], d));
+      for (int i = 0; i < U; ++i) {
+        uint32_t hi[2], lo[2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int n = n0 + i * WARPS;
-      // exponent of the maximum, kept where both the scale and its inverse are normal floats
-      int e = min(max(static_cast<int>(__float_as_uint(m[i]) >> 23) - 127, -110), 110);
-      if (m[i] == 0.f) e = 7;
-      const float up = __uint_as_float(static_cast<uint32_t>(127 + 7 - e) << 23);
-      const float x0 = __uint_as_float(u[i].x << 16) * up, x1 = __uint_as_float(u[i].x & 0xFFFF0000u) * up;
-      const float x2 = __uint_as_float(u[i].y << 16) * up, x3 = __uint_as_float(u[i].y & 0xFFFF0000u) * up;
-      const uint16_t c0 = e4m3x2_from_f32(x0, x1), c1 = e4m3x2_from_f32(x2, x3);
-      const float2 r0 = f32x2_from_e4m3x2(c0), r1 = f32x2_from_e4m3x2(c1);
-      const uint32_t lo = e4m3x2_from_f32(x0 - r0.x, x1 - r0.y) | static_cast<uint32_t>(e4m3x2_from_f32(x2 - r1.x, x3 - r1.y)) << 16;
-      if (n < PR) {
-        const int at = n * 128 + (((lane >> 2) ^ (n & 7)) << 4) + (lane & 3) * 4;
-        *reinterpret_cast<uint32_t*>(qh + at) = c0 | static_cast<uint32_t>(c1) << 16;
-        *reinterpret_cast<uint32_t*>(ql + at) = lo;
-        if (lane == 0) rows.unscale[n] = a.scale * kLog2e * __uint_as_float(static_cast<uint32_t>(127 + e - 7) << 23);
+        for (int k = 0; k < 2; ++k) {
+          const uint32_t p = k == 0 ? u[i].x : u[i].z, q = k == 0 ? u[i].y : u[i].w;
+          const float x0 = __uint_as_float(p << 16) * up, x1 = __uint_as_float(p & 0xFFFF0000u) * up;
+          const float x2 = __uint_as_float(q << 16) * up, x3 = __uint_as_float(q & 0xFFFF0000u) * up;
+          const uint16_t c0 = e4m3x2_from_f32(x0, x1), c1 = e4m3x2_from_f32(x2, x3);
+          const float2 r0 = f32x2_from_e4m3x2(c0), r1 = f32x2_from_e4m3x2(c1);
+          hi[k] = c0 | static_cast<uint32_t>(c1) << 16;
+          lo[k] = e4m3x2_from_f32(x0 - r0.x, x1 - r0.y) | static_cast<uint32_t>(e4m3x2_from_f32(x2 - r1.x, x3 - r1.y)) << 16;
+        }
+        const int c = part * U + i, at = n * 128 + (((c >> 1) ^ (n & 7)) << 4) + (c & 1) * 8;
+        *reinterpret_cast<uint2*>(qh + at) = make_uint2(hi[0], hi[1]);
+        *reinterpret_cast<uint2*>(ql + at) = make_uint2(lo[0], lo[1]);
       }
+    }
+    if (part == 0) {
+      rows.unscale[n] = a.scale * kLog2e * __uint_as_float(static_cast<uint32_t>(127 + e - 7) << 23);
+      rows.out[n] = (it.tok0 + t) * a.hq + h;
+      rows.lim[n] = n < it.rows ? min(it.key1, paged_key_limit(it.len, it.start + t, a.causal_block)) : it.key1;
     }
   }
   fence_proxy_async_smem();

@@ -296,7 +296,7 @@ __device__ __forceinline__ void run(const PagedAttnArgs& a, const CUtensorMap& t
   } else if (warp >= 4) {
     set_registers<kRegsSoftmax, true>();
     if (threadIdx.x - 128 < N) b.base[threadIdx.x - 128] = 0.f;
-    paged_stage_queries<N, 8, true>(a, it, sq, sq + N * kHd, b.rows, threadIdx.x - 128, 2);
+    paged_stage_queries<N, true>(a, it, sq, sq + N * kHd, b.rows, threadIdx.x - 128);
     if (lane == 0) mbar_arrive(&b.q_ready);
     named_sync(2, 256);
     // ---------------- softmax: a key a thread, half the columns a warpgroup ----------------

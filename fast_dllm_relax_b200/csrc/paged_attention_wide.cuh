@@ -109,7 +109,7 @@ __device__ __forceinline__ void run(const PagedAttnArgs& a, const CUtensorMap& t
   const int n_tiles = (it.key1 - it.key0 + kKeys - 1) / kKeys;
 
   if (warp >= 4) {
-    paged_stage_queries<kRows, 8, false>(a, it, smem + kOffQ, smem + kOffQ + kQ, b.rows, threadIdx.x - 128, 2);
+    paged_stage_queries<kRows, false>(a, it, smem + kOffQ, smem + kOffQ + kQ, b.rows, threadIdx.x - 128);
     if (lane == 0) mbar_arrive(&b.q_ready);
     named_sync(2, 256);
   }
