@@ -57,7 +57,8 @@ __device__ __forceinline__ void load8<float>(const float* p, float (&x)[8]) {
   x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
 }
 __device__ __forceinline__ void store8(bf16* p, const float (&x)[8]) {
-  *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
+  *reinterpret_cast<uint4*>(p) =
+      make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
 }
 __device__ __forceinline__ void store8(float* p, const float (&x)[8]) {
   reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
@@ -95,8 +96,9 @@ __device__ __forceinline__ float page_scale(float amax, bool keeps, float s_old,
   return keeps && s_old > s ? s_old : s;
 }
 
+// 64 registers: 1024 threads an SM, whose loads cover the latency of a unit's own chain (plan, page id, rows, maximum).
 template <typename T, typename TT>
-__global__ void __launch_bounds__(512) paged_append_kernel(const PagedAppendArgs a) {
+__global__ void __launch_bounds__(512, 2) paged_append_kernel(const PagedAppendArgs a) {
   __shared__ float red[16];
   pdl_trigger();
   pdl_wait();
@@ -122,7 +124,7 @@ __global__ void __launch_bounds__(512) paged_append_kernel(const PagedAppendArgs
       load8<TT>(sin_t + at, s);
       const T* src = static_cast<const T*>(a.q_in) + static_cast<size_t>(tok) * a.ldq + d;
       T* dst = static_cast<T*>(a.q_out) + static_cast<size_t>(tok) * a.hq * hd + d;
-#pragma unroll 4
+#pragma unroll 2
       for (int h = g % split; h < a.hq; h += split) {
         float x[8], y[8];
         load8<T>(src + h * hd, x);
