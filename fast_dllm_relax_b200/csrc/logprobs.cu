@@ -448,7 +448,7 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_kernel(const LogprobArgs
 }  // namespace
 
 // Parts of a row (at most kMaxParts) and chunks a part: what takes the fewest chunk times, waves of four CTAs an SM by
-// the chunks of a part and about two more for its bound, its ranking and the join.  (256 x 151936 fp32, top 5: 3 parts
+// the chunks of a part and about four more for its bound, its ranking and the join.  (256 x 151936 fp32, top 5: 3 parts
 // in two waves 40.0 us, 2 in one 36.4; 32 rows: 19 parts 14.3, 18 in one wave 13.8.)
 int logprobs_parts(int rows, int vocab, int dtype, int num_sms, int* part_chunks) {
   const int v = dtype == 1 ? Vec<bf16>::N : Vec<float>::N;
@@ -459,7 +459,7 @@ int logprobs_parts(int rows, int vocab, int dtype, int num_sms, int* part_chunks
   for (int p = 1; p <= std::min(chunks, kMaxParts); ++p) {
     const int each = (chunks + p - 1) / p;
     if ((chunks + each - 1) / each != p) continue;
-    const long long cost = (static_cast<long long>(rows) * p + slots - 1) / slots * (each + 2);
+    const long long cost = (static_cast<long long>(rows) * p + slots - 1) / slots * (each + 4);
     if (least < 0 || cost < least) least = cost, best = p;
   }
   *part_chunks = (chunks + best - 1) / best;
