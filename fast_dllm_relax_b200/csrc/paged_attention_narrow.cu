@@ -164,24 +164,30 @@ __device__ __forceinline__ void run(const PagedAttnArgs& a, const CUtensorMap& t
   }
   if (warp < kWarps) {
     // queries: f16 rows scaled by a power of two that puts the largest element into [2^7, 2^8)
-    for (int i = warp; i < R; i += kWarps) {
-      const int row = it.row0 + i;
-      const bool ok = i < it.rows;
-      const bf16* src = static_cast<const bf16*>(a.q) + static_cast<size_t>(it.tok0 + (ok ? row / G : 0)) * a.ldq +
-                        static_cast<size_t>(it.head * G + (ok ? row % G : 0)) * HD;
-      float x[HD / 32], m = 0.f;
+    float x[R / kWarps][HD / 32];  // a warp's rows together: one latency
 #pragma unroll
-      for (int j = 0; j < HD / 32; ++j) {
-        x[j] = ok ? to_f<bf16>(src[lane + 32 * j]) : 0.f;
-        m = fmaxf(m, fabsf(x[j]));
-      }
+    for (int k = 0; k < R / kWarps; ++k) {
+      const int i = warp + k * kWarps, row = it.row0 + min(i, it.rows - 1), t = row / G;
+      const bf16* src = static_cast<const bf16*>(a.q) + static_cast<size_t>(it.tok0 + t) * a.ldq +
+                        static_cast<size_t>(it.head * G + row - t * G) * HD;
+#pragma unroll
+      for (int j = 0; j < HD / 32; ++j) x[k][j] = i < it.rows ? to_f<bf16>(src[lane + 32 * j]) : 0.f;
+    }
+#pragma unroll
+    for (int k = 0; k < R / kWarps; ++k) {
+      const int i = warp + k * kWarps;
+      float m = 0.f;
+#pragma unroll
+      for (int j = 0; j < HD / 32; ++j) m = fmaxf(m, fabsf(x[k][j]));
+#pragma unroll
       for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
       // exponent of m, kept where both the scale and its inverse are normal floats
-      const int e = min(max(static_cast<int>(__float_as_uint(m) >> 23) - 127, -110), 110);
-      const float up = m > 0.f ? __uint_as_float(static_cast<uint32_t>(127 + 7 - e) << 23) : 1.f;
+      int e = min(max(static_cast<int>(__float_as_uint(m) >> 23) - 127, -110), 110);
+      if (m == 0.f) e = 7;
+      const float up = __uint_as_float(static_cast<uint32_t>(127 + 7 - e) << 23);
 #pragma unroll
-      for (int j = 0; j < HD / 32; ++j) sq[i * (HD + 8) + lane + 32 * j] = __float2half_rn(x[j] * up);
-      if (lane == 0) s_unscale[i] = a.scale * kLog2e / up;
+      for (int j = 0; j < HD / 32; ++j) sq[i * (HD + 8) + lane + 32 * j] = __float2half_rn(x[k][j] * up);
+      if (lane == 0) s_unscale[i] = a.scale * kLog2e * __uint_as_float(static_cast<uint32_t>(127 + e - 7) << 23);
     }
     named_sync(1, 32 * kWarps);
     uint32_t qf[KS][NT][2];  // B fragments: columns are query rows, the reduction order is the K fragment's
@@ -366,6 +372,7 @@ __device__ __forceinline__ void run(const PagedAttnArgs& a, const CUtensorMap& t
   __threadfence();
   constexpr int kPart = R * C4 + R;
   const float4* first = part - static_cast<size_t>(it.split) * kPart;
+#pragma unroll 1
   for (int i = threadIdx.x; i < it.rows * C4; i += 32 * (kWarps + 1)) {
     const int row = i / C4, c4 = i % C4;
     float m = -INFINITY;
