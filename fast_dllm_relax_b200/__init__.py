@@ -1,6 +1,7 @@
 """sm_100a (B200) library for Fast-dLLM v2 block-diffusion decoding.
 
     fast_dllm_relax_b200.engine.Engine     the nine entry points + fused extensions over torch tensors
+    fast_dllm_relax_b200.paged             page pool and plans of the paged 8-bit KV cache
     fast_dllm_relax_b200.artifacts         artifact directories (npz params, names, dtype, manifests)
     fast_dllm_relax_b200.vm_backend        vm[name] entry points for the TVM stand-in
     fast_dllm_relax_b200/tvm_shim/tvm      the TVM stand-in the reference's runtime imports

@@ -12,10 +12,13 @@
 //     of 4-thread groups is a lower bound of its `top`-th largest logit.  Later logits matter only when
 //     they exceed that bound (at equality the earlier ids win), so a chunk costs one compare a thread, and
 //     the few that pass are ranked against each other by counting: after 2, 4, 8, .. chunks, when the bound
-//     moves to the `top`-th largest so far, and at the end.  A part with more candidates than the buffer holds (many equal
-//     logits, ascending logits) is read again and extracted in order, `top` rounds a chunk at most.
+//     moves to the `top`-th largest so far, and at the end.  A part with more candidates than the buffer holds (many
+//     equal logits, ascending logits) is read again and extracted in order, `top` rounds a chunk at most.
 // The last CTA of a row (an arrival counter) joins the parts' statistics in part order and merges their
 // sorted lists, so one launch serves any split and the result does not depend on the arrival order.
+//
+// Measured, fp32, 151936 logits a row, five alternatives: 1024 rows 107 us, 5.8 TB/s; 256 rows 36.2 us, 4.3 TB/s (512
+// CTAs, one wave); one row 9.3 us (38 CTAs: latency of a chunk, its ranking and the join).
 #include <algorithm>
 
 #include "paged.h"

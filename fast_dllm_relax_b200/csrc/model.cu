@@ -1175,6 +1175,9 @@ long long fdllm_workspace_bytes(fdllm_handle* h) {
   for (auto* b : {&h->err, &h->tok_req, &h->tok_pos, &h->tok_row, &h->tmp_ids, &h->targets, &h->dec.ids,
                   &h->dec.block, &h->dec.cids, &h->dec.out})
     t += static_cast<long long>(b->bytes());
+  for (size_t n : {h->paged_qkv.bytes(), h->paged_part.bytes(), h->paged_ctr.bytes(), h->logprob_part.bytes(),
+                   h->logprob_keys.bytes(), h->logprob_ctr.bytes()})
+    t += static_cast<long long>(n);
   return t + static_cast<long long>(h->reqs.bytes());
 }
 

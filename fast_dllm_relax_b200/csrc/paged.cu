@@ -75,7 +75,8 @@ int check_paged(const fdllm_handle* h, const fdllm_paged_cache* c, int layer, co
 }
 
 // A share costs its prologue and its part of the join, more with more rows: 256 keys at least for up to 16 rows
-// (one token over 4000 keys: 9.2 us, 11.0 with 512), 512 above (8 rows over 392 keys: 12.2 us, 15.4 with 256).
+// (one token over 4000 keys: 8.9 us, 10.7 with 512), 512 above (8 requests of 8 rows over 4096 keys, 12/2 heads: 19.8
+// us, 21.9 with 256 and 23.8 with 1024).
 constexpr int kMinShareFew = 256, kMinShareMany = 512;
 constexpr int kShareUnit = 128;
 

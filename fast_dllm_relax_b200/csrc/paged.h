@@ -48,8 +48,8 @@ struct alignas(16) PagedItem {
 };
 static_assert(sizeof(PagedItem) == 4 * kPagedItemWords, "plan item layout");
 
-// Item classes, the largest tiles first in the plan: tiles of 16, 32 and 48 query rows (keys on the MMA's M side) and of up to 128 (rows
-// on it) at head_dim 128, of 8, 16 and 24 at the others (mma.sync).
+// Item classes, the largest tiles first in the plan: tiles of 16, 32 and 48 query rows (keys on the MMA's M side) and of
+// up to 128 (rows on it) at head_dim 128, of 8, 16 and 24 at the others (mma.sync).
 constexpr int kPagedClasses = 4;
 constexpr int kPagedWide = 3;
 constexpr int kPagedNarrowCtas = 3;  // CTAs on an SM at the other head sizes

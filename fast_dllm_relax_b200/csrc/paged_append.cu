@@ -16,6 +16,8 @@
 //     the CTA, and coded from the registers;
 //   - up to 16 token rows of one request for the queries: a thread holds its position's 8 cosines and sines and
 //     applies them to every head of its share.
+// Measured: 8 prompts of 4096 tokens, 12/2 heads of 128, bf16, 254 MB: 50.8 us, 5.0 TB/s; with 84 registers a thread,
+// so 640 threads an SM, 55.7.  32 block steps of 32 rows 4.7 us, one token 2.4.
 #include <algorithm>
 
 #include "paged.h"
@@ -96,7 +98,7 @@ __device__ __forceinline__ float page_scale(float amax, bool keeps, float s_old,
   return keeps && s_old > s ? s_old : s;
 }
 
-// 64 registers: 1024 threads an SM, whose loads cover the latency of a unit's own chain (plan, page id, rows, maximum).
+// 64 registers: 1024 threads an SM, whose loads cover a unit's own chain of latencies (plan, page id, rows, maximum).
 template <typename T, typename TT>
 __global__ void __launch_bounds__(512, 2) paged_append_kernel(const PagedAppendArgs a) {
   __shared__ float red[16];

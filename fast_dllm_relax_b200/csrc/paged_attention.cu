@@ -6,8 +6,8 @@
 // sum l once per 32 keys, and then a lane holds HD / 32 of the head's columns:
 //   s_t = scale (q . k_t),  o = o 2^(m - m') + sum_t 2^(s_t - m') v_t   (base-2 exponents, fp32)
 // with the 32 value rows' loads in flight together.  The warps' (m, l, o) are joined through shared memory.
-// Bound by latency at the sizes it serves (parity checks): 4 requests of 8 rows over 384..512 keys, 12/2 heads of
-// 128, take 16.5 us; one key at a time with the warp's lanes over its columns took 89.
+// Bound by latency at the sizes it serves (parity checks): 4 requests of 8 to 32 rows over 65 to 515 keys, 4/2 heads
+// of 64, take 16.5 us; one key at a time with the warp's lanes over its columns took 89.
 #include "paged.h"
 
 namespace fdllm {

@@ -24,8 +24,12 @@
 // columns a thread.  S_{j+1} is computed while tile j is in the softmax, once its scores have been loaded.  Two
 // CTAs share an SM.
 //
-// A tile whose keys are split over several items joins them through the workspace as in
-// paged_attention_narrow.cu: the last item to arrive adds the partials in item order.
+// A tile whose keys are split over several items joins them through the workspace: the last item to arrive adds the
+// partials in item order (paged_join).
+//
+// Measured, 12/2 heads of 128: one token over 397 keys 8.3 us (a chain of latencies: item, page ids, scales, copies,
+// two products, the join), over 32000 keys 16.7; 64 tokens over 700 to 8191 keys 24.8 us, 4.1 TB/s (102 MB: each of
+// the 284 items waits through its prologue once, and they end unevenly); 8 rows of 8 requests over 4096 keys 19.8 us.
 #pragma once
 #include "paged_mma.cuh"
 

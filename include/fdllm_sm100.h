@@ -248,9 +248,9 @@ typedef struct fdllm_paged_cache {
   int32_t page_size;     /* 16, 32, 64 or 128 */
 } fdllm_paged_cache;
 
-/* A batch of requests over paged caches, laid out by fdllm_paged_plan for the kernels.  The caller
- * copies the plan's `words` int32 words to 16-byte aligned device memory once and hands both to any number of
- * append / attention calls (every layer of a step uses the same plan). */
+/* A batch of requests over paged caches, laid out by fdllm_paged_plan_batch for the kernels.  The
+ * caller copies the plan's `words` int32 words to 16-byte aligned device memory once and hands both to any
+ * number of append / attention calls (every layer of a step uses the same plan). */
 typedef struct fdllm_paged_plan {
   int32_t words;         /* int32 words of the device copy */
   int32_t n;             /* requests */

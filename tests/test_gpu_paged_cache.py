@@ -241,6 +241,13 @@ def test_attention_long_split_keys(rows, dtype):
     run_attention((12, 2, 128), dtype, 64, [rows], [6001], None, 0, seed=rows)
 
 
+@pytest.mark.parametrize("heads", [(12, 2, 128), (8, 1, 128), (4, 2, 64), (8, 8, 64)], ids=str)
+def test_attention_split_tiles_of_every_size_in_one_call(heads):
+    # tiles of all sizes with their keys cut into 2 to 12 shares, beside a request that ends in its first page
+    run_attention(heads, "bfloat16", 32, [1, 3, 5, 8, 11, 16, 21, 40, 2],
+                  [3071, 2500, 1900, 3300, 1025, 2047, 2600, 1500, 9], None, 0, seed=heads[0])
+
+
 @pytest.mark.parametrize("rows", [1, 32])
 @pytest.mark.parametrize("scale", [0.0, 1.0, -0.3])
 def test_attention_scales(scale, rows):
