@@ -123,13 +123,15 @@ int plan_items(const fdllm_handle* h, const std::vector<PagedReq>& reqs, int cau
       longest = std::max<long long>(longest, tiles.back().keys);
     }
   }
-  long long share = (work * heads / slots + kShareUnit) / kShareUnit * kShareUnit;
-  while (share < longest) {
+  // the least share, in units, whose items fit one wave; the longest tile's where none does
+  long long low = work * heads / slots / kShareUnit, high = (longest + kShareUnit - 1) / kShareUnit;
+  while (low + 1 < high) {
+    const long long mid = (low + high) / 2;
     long long items = 0;
-    for (const Tile& t : tiles) items += splits_of(t, share);
-    if (items * heads <= slots) break;
-    share += (share / 16 + kShareUnit) / kShareUnit * kShareUnit;
+    for (const Tile& t : tiles) items += splits_of(t, mid * kShareUnit);
+    (items * heads <= slots ? high : low) = mid;
   }
+  const long long share = high * kShareUnit;
   for (size_t i = 0; i < reqs.size(); ++i) {
     const PagedReq& r = reqs[i];
     const long long rows = static_cast<long long>(r.rows) * G;
