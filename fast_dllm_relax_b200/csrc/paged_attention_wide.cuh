@@ -47,6 +47,7 @@ constexpr float kTrip = 15.f, kSeat = 8.f;
 constexpr int kRegsMisc = 48, kRegsSoftmax = 144, kRegsWiden = 48;
 static_assert(kRegsMisc + kRegsSoftmax + kRegsWiden == 3 * kRegsLaunch, "the split is the launch's registers");
 static_assert(2 * (kBytes + 2048) <= 228 * 1024, "two CTAs per SM");
+static_assert(kRows * kHd * 4 <= kOffV16, "O over the queries and the rings");
 
 // Instruction descriptors, fp32 accumulator, M 128: S (kind::f8f6f4, e4m3, K-major) and O (kind::f16, f16, A in
 // TMEM, B MN-major).
@@ -364,32 +365,30 @@ __device__ __forceinline__ void run(const PagedAttnArgs& a, const CUtensorMap& t
     ok = __all_sync(0xffffffffu, ok && mbar_wait(&b.o_final, 0));
     if (!ok && lane == 0) report_wait(a.err, kErrTimeoutEpilogue, 59, a.total_rows, it.splits);
     tc_fence_after_sync();
-    // a split tile leaves its partial: [128][128], then [128] (base, sum)
+    // O into shared memory, 16-byte units xor row mod 8 (the queries and the rings are done with): bf16, or fp32 for a
+    // partial; every warp then writes whole rows.
     const float inv = it.splits > 1 ? 1.f : l != 0.f ? 1.f / l : 0.f;
-    uint4* out = reinterpret_cast<uint4*>(static_cast<bf16*>(a.out) + static_cast<size_t>(b.rows.out[tid]) * kHd);
-    float4* part = a.part + it.part;
 #pragma unroll 1
     for (int c0 = 0; c0 < kHd; c0 += 32) {
       uint32_t v[32];
       tmem_ld_32x32b_x32(tmem + lane_base + kTmemO + c0, v);
       tmem_ld_wait();
       after_wait(v);
-      if (!valid) continue;
       auto at = [&](int c) { return __uint_as_float(v[c]) * inv; };
       if (it.splits == 1) {
 #pragma unroll
         for (int c = 0; c < 4; ++c)
-          out[c0 / 8 + c] = make_uint4(pack_bf16x2(at(8 * c), at(8 * c + 1)), pack_bf16x2(at(8 * c + 2), at(8 * c + 3)),
-                                       pack_bf16x2(at(8 * c + 4), at(8 * c + 5)), pack_bf16x2(at(8 * c + 6), at(8 * c + 7)));
+          *reinterpret_cast<uint4*>(smem + tid * 256 + (((c0 / 8 + c) ^ (tid & 7)) << 4)) =
+              make_uint4(pack_bf16x2(at(8 * c), at(8 * c + 1)), pack_bf16x2(at(8 * c + 2), at(8 * c + 3)),
+                         pack_bf16x2(at(8 * c + 4), at(8 * c + 5)), pack_bf16x2(at(8 * c + 6), at(8 * c + 7)));
       } else {
 #pragma unroll
         for (int c = 0; c < 8; ++c)
-          part[tid * (kHd / 4) + c0 / 4 + c] = make_float4(at(4 * c), at(4 * c + 1), at(4 * c + 2), at(4 * c + 3));
+          *reinterpret_cast<float4*>(smem + tid * 512 + (((c0 / 4 + c) ^ (tid & 7)) << 4)) =
+              make_float4(at(4 * c), at(4 * c + 1), at(4 * c + 2), at(4 * c + 3));
       }
     }
-    if (it.splits > 1) {
-      if (valid) reinterpret_cast<float2*>(part + kRows * (kHd / 4))[tid] = make_float2(base, l);
-    }
+    if (it.splits > 1 && valid) reinterpret_cast<float2*>(a.part + it.part + kRows * (kHd / 4))[tid] = make_float2(base, l);
     tc_fence_before_sync();
   }
   __syncwarp();
@@ -403,7 +402,20 @@ __device__ __forceinline__ void run(const PagedAttnArgs& a, const CUtensorMap& t
     tc_fence_after_sync();
     tmem_dealloc(tmem, kTmemCols);
   }
-  if (it.splits > 1) paged_join<kRows, kThreads>(a, it, b.rows.out, smem);
+  if (it.splits == 1) {
+    for (int i = threadIdx.x; i < it.rows * 16; i += kThreads) {
+      const int row = i >> 4, c = i & 15;
+      reinterpret_cast<uint4*>(static_cast<bf16*>(a.out) + static_cast<size_t>(b.rows.out[row]) * kHd)[c] =
+          *reinterpret_cast<const uint4*>(smem + row * 256 + ((c ^ (row & 7)) << 4));
+    }
+    return;
+  }
+  // a split tile leaves its partial: [128][128], then [128] (base, sum)
+  for (int i = threadIdx.x; i < it.rows * 32; i += kThreads) {
+    const int row = i >> 5, c = i & 31;
+    a.part[it.part + i] = *reinterpret_cast<const float4*>(smem + row * 512 + ((c ^ (row & 7)) << 4));
+  }
+  paged_join<kRows, kThreads>(a, it, b.rows.out, smem);
 }
 
 }  // namespace paged_wide
