@@ -20,13 +20,13 @@
 // products.
 //
 // Measured, 12/2 heads of 128: 2 prompts of 4096 tokens, block-causal, 135 us, 770 TFLOP/s of the formula's two
-// products; 32 block steps of 32 rows over 512 to 1024 keys 24.6 us, 8 over 4096 keys 33.2.
+// products; 32 block steps of 32 rows over 512 to 1024 keys 22.8 us, 8 over 4096 keys 29.7.
 //
 // What bounds it: no one pipe.  A tile of 8192 scores takes 1100 clocks of an SM, of which the tensor pipes are busy
 // 650 (Q is read twice for S, at 64 bytes a clock), the exponentials 512 and shared memory 812 (104 KB); the chain
 // S, softmax, P, O of two CTAs does not keep any of them full, and 768 items' prologues and epilogues are a fifth of
 // the prompts' time.  What did not shorten it: S of two tiles in one product (159 us), half a row a thread on eight
-// softmax warps (134.5), one S and two P buffers (141).
+// softmax warps (134.5), one S and two P buffers (140), that with Qh in TMEM (147).
 //
 // A tile whose keys are split over several items joins them through the workspace: the last item to arrive adds the
 // partials in item order (paged_join).
