@@ -75,7 +75,7 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
 
 struct Bars {
   uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
-  uint64_t scale_full[4], q_ready, s_full[2], p_full[2], w_full[2], pv_done[2], o_final;
+  uint64_t q_ready, s_full[2], p_full[2], w_full[2], pv_done[2], o_final;
   uint32_t tmem;
   PagedRows<kRows> rows;
   float4 scale[4][kKeys / 16];  // of tile j & 3, its 16-key groups: ks, log2 vs, 1 / vs
@@ -91,12 +91,11 @@ __device__ __forceinline__ void run(const PagedAttnArgs& a, const CUtensorMap& t
       mbar_init(&b.k_empty[i], 1);
       mbar_init(&b.v_full[i], 32);
       mbar_init(&b.v_empty[i], 4);
-      mbar_init(&b.s_full[i], 1);
+      mbar_init(&b.s_full[i], 2);
       mbar_init(&b.p_full[i], 4);
       mbar_init(&b.w_full[i], 4);
       mbar_init(&b.pv_done[i], 1);
     }
-    for (int i = 0; i < 4; ++i) mbar_init(&b.scale_full[i], 1);
     mbar_init(&b.q_ready, 8);
     mbar_init(&b.o_final, 1);
     mbar_fence_init();
@@ -157,7 +156,7 @@ __device__ __forceinline__ void run(const PagedAttnArgs& a, const CUtensorMap& t
       }
       if (live) load(&tm_k, &b.k_full[st], smem + kOffK + st * kTile);
       // the scales of the tile's 16-key groups.  Slot j & 3: S_{j-2} is done, so P_{j-4} is used and its softmax past.
-      // A barrier of their own: K's may be two phases on before the softmax comes to this tile.
+      // They reach the softmax through the MMA issuer, which waits for K and arrives for S (a wait costs 100 clocks).
       const int group_page = page0 - batch + ((16 * (lane & 3)) >> a.page_shift);
       const float kg = __shfl_sync(0xffffffffu, ks, group_page), vg = __shfl_sync(0xffffffffu, vs, group_page);
       if (lane < 4) {
@@ -165,7 +164,6 @@ __device__ __forceinline__ void run(const PagedAttnArgs& a, const CUtensorMap& t
         b.scale[j & 3][lane] = make_float4(kg, lv, exp2_approx(-lv), 0.f);
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(&b.scale_full[j & 3]);
       mbar_arrive(&b.k_full[st]);
       if (!__all_sync(0xffffffffu, mbar_wait(&b.v_empty[st], free_parity))) {
         report_wait(a.err, kErrTimeoutProducer, 52, a.total_rows, it.splits);
@@ -203,6 +201,7 @@ __device__ __forceinline__ void run(const PagedAttnArgs& a, const CUtensorMap& t
             mma_f8(tmem + kTmemS + st * kKeys, ql + 2 * k, kd + 2 * k, kIdescS, 1u);
           }
           tc_commit(&b.s_full[st]);
+          mbar_arrive(&b.s_full[st]);  // releases the scales
           tc_commit(&b.k_empty[st]);
         }
         if (j >= 1) {  // O += P_i V_i, i = j - 1
@@ -281,7 +280,7 @@ __device__ __forceinline__ void run(const PagedAttnArgs& a, const CUtensorMap& t
     bool ok = true, seated = false;  // seated: the base has been set (the row has attended a key)
     for (int j = 0; j < n_tiles; ++j) {
       const int sb = j & 1, key0 = it.key0 + j * kKeys;
-      ok = __all_sync(0xffffffffu, mbar_wait(&b.scale_full[j & 3], (j >> 2) & 1u) && mbar_wait(&b.s_full[sb], (j >> 1) & 1u));
+      ok = __all_sync(0xffffffffu, mbar_wait(&b.s_full[sb], (j >> 1) & 1u));
       if (!ok) break;
       if (q4 * 32 >= it.rows) {  // only padding rows: whatever P holds there stays in their rows of O
         if (lane == 0) mbar_arrive(&b.p_full[sb]);
