@@ -75,7 +75,7 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
 
 struct Bars {
   uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
-  uint64_t q_ready, s_full[2], p_full[2], w_full[2], pv_done[2], o_final;
+  uint64_t q_ready, s_full[2], pv_ready[2], pv_done[2], o_final;  // pv_ready: P and the widened V
   uint32_t tmem;
   PagedRows<kRows> rows;
   float4 scale[4][kKeys / 16];  // of tile j & 3, its 16-key groups: ks, log2 vs, 1 / vs
@@ -92,8 +92,7 @@ __device__ __forceinline__ void run(const PagedAttnArgs& a, const CUtensorMap& t
       mbar_init(&b.v_full[i], 32);
       mbar_init(&b.v_empty[i], 4);
       mbar_init(&b.s_full[i], 2);
-      mbar_init(&b.p_full[i], 4);
-      mbar_init(&b.w_full[i], 4);
+      mbar_init(&b.pv_ready[i], 8);
       mbar_init(&b.pv_done[i], 1);
     }
     mbar_init(&b.q_ready, 8);
@@ -206,12 +205,8 @@ __device__ __forceinline__ void run(const PagedAttnArgs& a, const CUtensorMap& t
         }
         if (j >= 1) {  // O += P_i V_i, i = j - 1
           const int i = j - 1, buf = i & 1;
-          if (!mbar_wait(&b.w_full[buf], (i >> 1) & 1u)) {
+          if (!mbar_wait(&b.pv_ready[buf], (i >> 1) & 1u)) {
             site = 56;
-            break;
-          }
-          if (!mbar_wait(&b.p_full[buf], (i >> 1) & 1u)) {
-            site = 57;
             break;
           }
           tc_fence_after_sync();
@@ -265,7 +260,7 @@ __device__ __forceinline__ void run(const PagedAttnArgs& a, const CUtensorMap& t
       }
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&b.w_full[st]);
+      if (lane == 0) mbar_arrive(&b.pv_ready[st]);
     }
     if (!ok && lane == 0) report_wait(a.err, kErrTimeoutEpilogue, 58, a.total_rows, it.splits);
   } else if (warp >= 4) {
@@ -283,7 +278,7 @@ __device__ __forceinline__ void run(const PagedAttnArgs& a, const CUtensorMap& t
       ok = __all_sync(0xffffffffu, mbar_wait(&b.s_full[sb], (j >> 1) & 1u));
       if (!ok) break;
       if (q4 * 32 >= it.rows) {  // only padding rows: whatever P holds there stays in their rows of O
-        if (lane == 0) mbar_arrive(&b.p_full[sb]);
+        if (lane == 0) mbar_arrive(&b.pv_ready[sb]);
         continue;
       }
       tc_fence_after_sync();
@@ -359,7 +354,7 @@ __device__ __forceinline__ void run(const PagedAttnArgs& a, const CUtensorMap& t
       tmem_st_wait();
       tc_fence_before_sync();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&b.p_full[sb]);
+      if (lane == 0) mbar_arrive(&b.pv_ready[sb]);
     }
     ok = __all_sync(0xffffffffu, ok && mbar_wait(&b.o_final, 0));
     if (!ok && lane == 0) report_wait(a.err, kErrTimeoutEpilogue, 59, a.total_rows, it.splits);
