@@ -68,6 +68,11 @@ int check_paged(const fdllm_handle* h, const fdllm_paged_cache* c, int layer, co
   if (table_ld < p->table_cols)
     return fail(FDLLM_ERR_INVALID, "page table has " + std::to_string(table_ld) + " columns; the longest request needs " +
                                        std::to_string(p->table_cols));
+  const fdllm_config& cfg = h->cfg;
+  if (const int32_t* s = p->priv + kPagedShape; s[0] != cfg.num_attention_heads || s[1] != cfg.num_key_value_heads ||
+                                                s[2] != cfg.head_dim || s[3] != h->dtype)
+    return fail(FDLLM_ERR_INVALID, "the plan was laid out for " + std::to_string(s[0]) + "/" + std::to_string(s[1]) +
+                                       " heads of " + std::to_string(s[2]) + " in another handle");
   const size_t heads = static_cast<size_t>(c->pages) * h->cfg.num_key_value_heads;
   *layer_scales = static_cast<size_t>(layer) * heads;
   *layer_codes = static_cast<size_t>(layer) * heads * c->page_size * h->cfg.head_dim;
@@ -323,6 +328,8 @@ int fdllm_paged_plan_batch(fdllm_handle* h, const int32_t* rows, const int32_t* 
     out.causal_block = causal_block;
     out.table_cols = static_cast<int>((max_len + page_size - 1) / page_size);
     out.max_position = static_cast<int>(max_pos);
+    const int32_t shape[4] = {h->cfg.num_attention_heads, h->cfg.num_key_value_heads, h->cfg.head_dim, h->dtype};
+    std::copy(shape, shape + 4, out.priv + kPagedShape);
     int at = n * kPagedReqWords;
     out.priv[kPagedPageUnits] = static_cast<int>(units.size());
     out.priv[kPagedPageOff] = at;

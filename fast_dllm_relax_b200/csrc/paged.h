@@ -64,7 +64,8 @@ enum PagedPriv : int {
   kPagedItemOff = kPagedItems + kPagedClasses,  // word offset of the items, class after class from the last
   kPagedQUnits,         // number of query units
   kPagedQOff,           // word offset of the query units
-  kPagedPrivEnd,
+  kPagedShape,          // [4] the handle's heads, KV heads, head_dim and dtype
+  kPagedPrivEnd = kPagedShape + 4,
 };
 
 struct PagedAppendArgs {

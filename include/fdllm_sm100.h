@@ -250,7 +250,8 @@ typedef struct fdllm_paged_cache {
 
 /* A batch of requests over paged caches, laid out by fdllm_paged_plan_batch for the kernels.  The
  * caller copies the plan's `words` int32 words to 16-byte aligned device memory once and hands both to any
- * number of append / attention calls (every layer of a step uses the same plan). */
+ * number of append / attention calls (every layer of a step uses the same plan) of the handle that laid it
+ * out or of another with the same heads and dtype. */
 typedef struct fdllm_paged_plan {
   int32_t words;         /* int32 words of the device copy */
   int32_t n;             /* requests */

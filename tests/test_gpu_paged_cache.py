@@ -404,6 +404,20 @@ def test_refusals():
     assert eng.device_error() == 0
 
 
+@pytest.mark.parametrize("other", [((8, 1, 128), "bfloat16"), ((16, 4, 128), "bfloat16"), ((4, 2, 64), "bfloat16"),
+                                   ((12, 2, 128), "float32")], ids=str)
+def test_a_plan_for_other_heads_or_another_type_is_refused(other):
+    eng = engine((12, 2, 128), "bfloat16")
+    plan = engine(*other).paged_plan([8], [40])
+    cache = eng.new_paged_cache(4, layers=1)
+    table = torch.zeros(1, 2, dtype=torch.int32, device="cuda")
+    q = torch.zeros(8, 1536, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(ValueError, match="laid out for"):
+        eng.paged_attention(cache, 0, plan, table, q)
+    with pytest.raises(ValueError, match="laid out for"):
+        eng.paged_append(cache, 0, plan, table, q, q[:, :256], q[:, :256])
+
+
 def test_unaligned_rows_are_copied():
     eng = engine((12, 2, 128), "bfloat16")
     gen = torch.Generator().manual_seed(8)
