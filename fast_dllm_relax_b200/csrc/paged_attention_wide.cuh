@@ -74,7 +74,7 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
 }
 
 struct Bars {
-  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
+  uint64_t k_full[2], v_full[2], v_empty[2];
   uint64_t q_ready, s_full[2], pv_ready[2], pv_done[2], o_final;  // pv_ready: P and the widened V
   uint32_t tmem;
   PagedRows<kRows> rows;
@@ -88,7 +88,6 @@ __device__ __forceinline__ void run(const PagedAttnArgs& a, const CUtensorMap& t
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&b.k_full[i], 32);
-      mbar_init(&b.k_empty[i], 1);
       mbar_init(&b.v_full[i], 32);
       mbar_init(&b.v_empty[i], 4);
       mbar_init(&b.s_full[i], 2);
@@ -149,7 +148,8 @@ __device__ __forceinline__ void run(const PagedAttnArgs& a, const CUtensorMap& t
                      : "memory");
         tma_load_2d(dst + lane * box * kHd, map, bar, 0, src, policy);
       };
-      if (!__all_sync(0xffffffffu, mbar_wait(&b.k_empty[st], free_parity))) {
+      // K_{j-2} has been used once S_{j-2} is there
+      if (j >= 2 && !__all_sync(0xffffffffu, mbar_wait(&b.s_full[st], free_parity))) {
         report_wait(a.err, kErrTimeoutProducer, 51, a.total_rows, it.splits);
         break;
       }
@@ -201,7 +201,6 @@ __device__ __forceinline__ void run(const PagedAttnArgs& a, const CUtensorMap& t
           }
           tc_commit(&b.s_full[st]);
           mbar_arrive(&b.s_full[st]);  // releases the scales
-          tc_commit(&b.k_empty[st]);
         }
         if (j >= 1) {  // O += P_i V_i, i = j - 1
           const int i = j - 1, buf = i & 1;
