@@ -14,8 +14,8 @@
 // sum takes it back out.
 //
 // Roles (384 threads, registers moved to the softmax): warp 0 the TMA producer (a lane a page; page ids and
-// scales 32 pages at a time), warp 1 the MMA issuer and TMEM owner, warps 4-7 the softmax, a row a thread,
-// warps 8-11 widen V.  S, P and the widened V are double-buffered: S_{j+1} and V_{j+1} are made while tile j is
+// scales 32 pages at a time), warp 1 issues S and owns TMEM, warp 2 issues P V (one thread for both took 128 us for
+// 123 below: an issue blocks while the tensor core is busy), warps 4-7 the softmax, a row a thread, warps 8-11 widen V.  S, P and the widened V are double-buffered: S_{j+1} and V_{j+1} are made while tile j is
 // in the softmax.  Two CTAs share an SM (256 TMEM columns and 97 KB each), so one's softmax covers the other's
 // products.
 //
@@ -177,48 +177,50 @@ __device__ __forceinline__ void run(const PagedAttnArgs& a, const CUtensorMap& t
       if (!mbar_wait(&b.k_full[j & 1], (j >> 1) & 1u) || !mbar_wait(&b.v_full[j & 1], (j >> 1) & 1u)) break;
   } else if (warp == 1) {
     if (lane == 0) {
-      // ---------------- MMA issuer ----------------
+      // ---------------- issuer of S_j = (Qh + Ql) K_j^T, into the buffer that P_{j-2} has left ----------------
       int site = 0;
       if (!mbar_wait(&b.q_ready, 0)) site = 53;
       const uint64_t qh = umma_desc_sw128(smem + kOffQ), ql = umma_desc_sw128(smem + kOffQ + kQ);
-      for (int j = 0; j <= n_tiles && site == 0; ++j) {
-        if (j < n_tiles) {  // S_j = (Qh + Ql) K_j^T, into the buffer that P_{j-2} has left
-          const int st = j & 1;
-          if (!mbar_wait(&b.k_full[st], (j >> 1) & 1u)) {
-            site = 54;
-            break;
-          }
-          if (j >= 2 && !mbar_wait(&b.pv_done[st], ((j - 2) >> 1) & 1u)) {
-            site = 55;
-            break;
-          }
-          tc_fence_after_sync();
-          const uint64_t kd = umma_desc_sw128(smem + kOffK + st * kTile);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            mma_f8(tmem + kTmemS + st * kKeys, qh + 2 * k, kd + 2 * k, kIdescS, k > 0 ? 1u : 0u);
-            mma_f8(tmem + kTmemS + st * kKeys, ql + 2 * k, kd + 2 * k, kIdescS, 1u);
-          }
-          tc_commit(&b.s_full[st]);
-          mbar_arrive(&b.s_full[st]);  // releases the scales
+      for (int j = 0; j < n_tiles && site == 0; ++j) {
+        const int st = j & 1;
+        if (!mbar_wait(&b.k_full[st], (j >> 1) & 1u)) {
+          site = 54;
+          break;
         }
-        if (j >= 1) {  // O += P_i V_i, i = j - 1
-          const int i = j - 1, buf = i & 1;
-          if (!mbar_wait(&b.pv_ready[buf], (i >> 1) & 1u)) {
-            site = 56;
-            break;
-          }
-          tc_fence_after_sync();
-#pragma unroll
-          for (int k = 0; k < 4; ++k)  // 16 keys a step: 8 columns of P, two 8-row groups of V
-            mma_f16_ta(tmem + kTmemO, tmem + kTmemS + buf * kKeys + 8 * k,
-                       umma_desc_sw128_mn(smem + kOffV16 + buf * kV16 + k * 2048, kV16 / 2, 1024), kIdescO,
-                       (i > 0 || k > 0) ? 1u : 0u);
-          tc_commit(&b.pv_done[buf]);
-          if (i == n_tiles - 1) tc_commit(&b.o_final);
+        if (j >= 2 && !mbar_wait(&b.pv_done[st], ((j - 2) >> 1) & 1u)) {
+          site = 55;
+          break;
         }
+        tc_fence_after_sync();
+        const uint64_t kd = umma_desc_sw128(smem + kOffK + st * kTile);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          mma_f8(tmem + kTmemS + st * kKeys, qh + 2 * k, kd + 2 * k, kIdescS, k > 0 ? 1u : 0u);
+          mma_f8(tmem + kTmemS + st * kKeys, ql + 2 * k, kd + 2 * k, kIdescS, 1u);
+        }
+        tc_commit(&b.s_full[st]);
+        mbar_arrive(&b.s_full[st]);  // releases the scales
       }
       if (site != 0) report_wait(a.err, kErrTimeoutMma, site, a.total_rows, it.splits);
+    }
+  } else if (warp == 2) {
+    if (lane == 0) {
+      // ---------------- issuer of O += P_j V_j ----------------
+      bool ok = true;
+      for (int j = 0; j < n_tiles && ok; ++j) {
+        const int buf = j & 1;
+        ok = mbar_wait(&b.pv_ready[buf], (j >> 1) & 1u);
+        if (!ok) break;
+        tc_fence_after_sync();
+#pragma unroll
+        for (int k = 0; k < 4; ++k)  // 16 keys a step: 8 columns of P, two 8-row groups of V
+          mma_f16_ta(tmem + kTmemO, tmem + kTmemS + buf * kKeys + 8 * k,
+                     umma_desc_sw128_mn(smem + kOffV16 + buf * kV16 + k * 2048, kV16 / 2, 1024), kIdescO,
+                     (j > 0 || k > 0) ? 1u : 0u);
+        tc_commit(&b.pv_done[buf]);
+        if (j == n_tiles - 1) tc_commit(&b.o_final);
+      }
+      if (!ok) report_wait(a.err, kErrTimeoutMma, 56, a.total_rows, it.splits);
     }
   } else if (warp >= 8) {
     set_registers<kRegsWiden, false>();
