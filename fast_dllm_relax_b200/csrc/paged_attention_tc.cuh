@@ -138,7 +138,7 @@ struct Cfg {
 template <int N>
 struct Bars {
   uint64_t k_full[3], k_empty[3], v_full[3], v_empty[3];
-  uint64_t q_ready, s_full, s_free, p_full, pv_done[2], o_final;
+  uint64_t q_ready, s_full, s_free, p_full[2], pv_done[2], o_final;
   uint32_t tmem;
   // of a stage's pages: log2 vs, 1 / vs, and ks over that of the first page of the 32 keys
   float4 scale[3][kKeys / 16];
@@ -170,7 +170,8 @@ __device__ __forceinline__ void run(const PagedAttnArgs& a, const CUtensorMap& t
     mbar_init(&b.q_ready, 8);
     mbar_init(&b.s_full, 1);
     mbar_init(&b.s_free, 8);
-    mbar_init(&b.p_full, 8);
+    mbar_init(&b.p_full[0], 8);
+    mbar_init(&b.p_full[1], 8);
     mbar_init(&b.pv_done[0], 1);
     mbar_init(&b.pv_done[1], 1);
     mbar_init(&b.o_final, 1);
@@ -280,7 +281,7 @@ __device__ __forceinline__ void run(const PagedAttnArgs& a, const CUtensorMap& t
         }
         if (j >= 1) {  // O^T += V_i^T (Pa | Pb | Pc)_i^T, i = j - 1
           const int i = j - 1, st = i % kStages;
-          if (!mbar_wait(&b.p_full, i & 1u)) {
+          if (!mbar_wait(&b.p_full[i & 1], (i >> 1) & 1u)) {
             site = 45;
             break;
           }
@@ -461,7 +462,7 @@ __device__ __forceinline__ void run(const PagedAttnArgs& a, const CUtensorMap& t
       }
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&b.p_full);
+      if (lane == 0) mbar_arrive(&b.p_full[j & 1]);
     }
 
     // row sums over the 128 keys
