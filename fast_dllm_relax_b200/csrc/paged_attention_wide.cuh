@@ -15,9 +15,9 @@
 //
 // Roles (384 threads, registers moved to the softmax): warp 0 the TMA producer (a lane a page; page ids and
 // scales 32 pages at a time), warp 1 issues S and owns TMEM, warp 2 issues P V (one thread for both took 128 us for
-// 123 below: an issue blocks while the tensor core is busy), warps 4-7 the softmax, a row a thread, warps 8-11 widen V.  S, P and the widened V are double-buffered: S_{j+1} and V_{j+1} are made while tile j is
-// in the softmax.  Two CTAs share an SM (256 TMEM columns and 97 KB each), so one's softmax covers the other's
-// products.
+// 123 below: an issue blocks while the tensor core is busy), warps 4-7 the softmax, a row a thread, warps 8-11 widen
+// V.  S, P and the widened V are double-buffered: S_{j+1} and V_{j+1} are made while tile j is in the softmax.  Two
+// CTAs share an SM (256 TMEM columns and 110 KB each), so one's softmax covers the other's products.
 //
 // Measured, 12/2 heads of 128: 2 prompts of 4096 tokens, block-causal, 123 us, 845 TFLOP/s of the formula's two
 // products; 32 block steps of 32 rows over 512 to 1024 keys 22.2 us, 8 over 4096 keys 28.7.
@@ -25,8 +25,9 @@
 // What bounds it: no one pipe.  A tile of 8192 scores takes 950 clocks of an SM, of which the tensor core with its
 // operand reads is busy 62 % (Q is read twice for S, at 64 bytes a clock), the exponentials 42 % and issue 57 %; the
 // chain S, softmax, P, O of two CTAs does not keep any of them full, each wait on a barrier in it costs 100 clocks, and
-// 768 items' prologues and epilogues are a fifth of the prompts' time.  What did not shorten it, of 134 us then: S of two tiles in one product (159), half a row a
-// thread on eight softmax warps (134.5), one S and two P buffers (140), that with Qh in TMEM (147).
+// 768 items' prologues and epilogues are a fifth of the prompts' time.  What did not shorten it, of 134 us then: S of
+// two tiles in one product (159), half a row a thread on eight softmax warps (134.5), one S and two P buffers (140),
+// that with Qh in TMEM (147).
 //
 // A tile whose keys are split over several items joins them through the workspace: the last item to arrive adds the
 // partials in item order (paged_join).
