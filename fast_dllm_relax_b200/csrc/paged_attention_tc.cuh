@@ -237,9 +237,9 @@ __device__ __forceinline__ void run(const PagedAttnArgs& a, const CUtensorMap& t
       // the tile's scales (V's stage is free: its softmax is long past)
       const float ks_j = __shfl_sync(0xffffffffu, ks, from), vs_j = __shfl_sync(0xffffffffu, sc.x, from);
       const float ks_0 = __shfl_sync(0xffffffffu, ks_j, lane & ~1);  // (pages of 16: two to 32 keys)
-      if (live) {
-        const float lv = __log2f(vs_j);
-        b.scale[st][lane] = make_float4(lv, exp2_approx(-lv), a.page_shift == 4 ? ks_j / ks_0 : 1.f, 0.f);
+      if (lane < per_tile) {  // a dead page's slot too: its keys' weights are 0, what multiplies them must be a number
+        const float lv = __log2f(live ? vs_j : 1.f);
+        b.scale[st][lane] = make_float4(lv, exp2_approx(-lv), a.page_shift == 4 && live ? ks_j / ks_0 : 1.f, 0.f);
       }
       if (j == 0 && !mbar_wait(&b.q_ready, 0))  // the queries' scales (the others' waits then expire too)
         report_wait(a.err, kErrTimeoutProducer, 50, a.total_rows, it.splits);
@@ -321,7 +321,7 @@ __device__ __forceinline__ void run(const PagedAttnArgs& a, const CUtensorMap& t
       const int st = j % kStages;
       const int key = it.key0 + j * kKeys + key_lane;
       ok = ok && mbar_wait(&b.v_full[st], (j / kStages) & 1u);
-      const float4 sc = b.scale[st][key_lane >> a.page_shift];  // (of a dead key's page: anything)
+      const float4 sc = b.scale[st][key_lane >> a.page_shift];
       ok = ok && mbar_wait(&b.s_full, j & 1u);
       __syncwarp();
       tc_fence_after_sync();
