@@ -6,7 +6,7 @@
 // plan, a tile of at most N rows and a range of keys, in tiles of 128 keys with the keys on the MMA's M side:
 //   S^T [128 keys, 2 N]    = K (Qh | Ql)^T          A: the K tile (e4m3, K-major), B: the queries (e4m3, K-major)
 //   P^T [128 keys, N]      = 2^(a S + log2 vs - B)
-//   O^T [128 columns, 3 N] += V^T (Pa | Pb | Pc)^T  A: the V tile (e4m3, MN-major), B: P (e4m3, MN-major)
+//   O^T [128 columns, 3 N] += V^T (Pa | Pb | Pc)^T  A: the V tile (e4m3, MN-major), B: P (e5m2, MN-major)
 // so a page goes from memory by TMA straight into both operands, N follows the number of query rows (a lone
 // token needs 16 columns, not 128 rows of padding), and a thread of the softmax holds one key: the page's scales
 // are one pair a thread.  What an SM pays a tile is shared-memory traffic (the tensor core reads A at 64 bytes a
@@ -14,10 +14,14 @@
 //
 // Precision.  A bf16 query has 8 significant bits: Q = Qh + Ql under one power of two per row (largest element
 // in [2^7, 2^8)), exact for elements above 2^-10 of the row's largest and to 2^-18 of it below.  A probability
-// is P = Pa + 2^-5 Pb + 2^-10 Pc, each term the e4m3 rounding of what the ones before leave: at least 8 bits for
-// weights down to 2^-14 of the largest, 4 bits to 2^-19.  Each column's base B moves only when a weight passes
-// 2^kTrip (then its maximum sits at 2^kSeat): one block-wide vote a tile instead of a maximum over 128 lanes.
-// log2 vs in the exponent keeps P in range whatever the page scales are; the row sums take it back out.
+// is rounded to f16, as for many rows, and split into P = Pa + 2^-3 Pb + 2^-8 Pc, each term the e5m2 rounding of what
+// the ones before leave.  e5m2 has f16's exponents and 3 of its 11 bits, and a signed remainder brings 4 with each
+// term, so the three hold every f16 from 2^-13 on and are 2^-24 off at most below: 11 bits for weights down to 2^-21 of
+// the largest (seated at 2^8 or more), then a bit less a power of two, the last lost at 2^-32.  (Three e4m3 terms hold
+// 12 bits at the top, but end at 2^-22 of a maximum at 2^3: beside a sink whose own value is small the weights left
+// over are the result.)  Each column's base B moves only when a weight passes 2^kTrip (then its maximum sits at
+// 2^kSeat): one block-wide vote a tile instead of a maximum over 128 lanes.  log2 vs in the exponent keeps P in range
+// whatever the page scales are; the row sums take it back out.
 //
 // Roles (384 threads, registers moved to the softmax): warp 0 the TMA producer (a lane a page; page ids and
 // scales 32 pages at a time), warp 1 the MMA issuer and TMEM owner, warps 4-11 the softmax, a key and half the
@@ -39,12 +43,12 @@ namespace paged_tc {
 constexpr int kKeys = 128;
 constexpr int kHd = 128;
 constexpr int kTile = kKeys * kHd;  // bytes of a K or V tile
-constexpr float kTrip = 8.f, kSeat = 3.f;
+constexpr float kTrip = 15.f, kSeat = 8.f;
 
-// Instruction descriptor, kind::f8f6f4: fp32 accumulator, both operands e4m3, M 128; S = K Q^T has both K-major,
-// O^T = V^T P^T both MN-major.
+// Instruction descriptor, kind::f8f6f4: fp32 accumulator, M 128; S = K Q^T has both operands e4m3 and K-major,
+// O^T = V^T P^T both MN-major and B e5m2.
 constexpr uint32_t idesc_s(int n) { return (1u << 4) | (static_cast<uint32_t>(n >> 3) << 17) | ((128u >> 4) << 24); }
-constexpr uint32_t idesc_o(int n) { return idesc_s(n) | (1u << 15) | (1u << 16); }
+constexpr uint32_t idesc_o(int n) { return idesc_s(n) | (1u << 10) | (1u << 15) | (1u << 16); }
 
 // Shared-memory descriptor of an unswizzled MN-major operand: core matrices of 8 K rows by 16 MN bytes
 // (128 B, row after row), `mn` bytes between core matrices along MN and `k` along K.
@@ -74,13 +78,15 @@ __device__ __forceinline__ void after_wait(uint32_t (&r)[8]) {
   for (int i = 0; i < 8; ++i) asm volatile("" : "+r"(r[i]));
 }
 
-__device__ __forceinline__ uint16_t e4m3x2_from_f16x2(__half2 h) {
+// float8 e5m2 (1 sign, 5 exponent, 2 mantissa bits): nearest even, and back (exact).
+__device__ __forceinline__ uint16_t e5m2x2_from_f16x2(__half2 h) {
   uint16_t r;
-  asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(r) : "r"(*reinterpret_cast<const uint32_t*>(&h)));
+  asm("cvt.rn.satfinite.e5m2x2.f16x2 %0, %1;" : "=h"(r) : "r"(*reinterpret_cast<const uint32_t*>(&h)));
   return r;
 }
-__device__ __forceinline__ __half2 half2_from_e4m3x2(uint16_t c) {
-  const uint32_t u = f16x2_from_e4m3x2(c);
+__device__ __forceinline__ __half2 half2_from_e5m2x2(uint16_t c) {
+  uint32_t u;
+  asm("cvt.rn.f16x2.e5m2x2 %0, %1;" : "=r"(u) : "h"(c));
   return *reinterpret_cast<const __half2*>(&u);
 }
 
@@ -439,12 +445,12 @@ __device__ __forceinline__ void run(const PagedAttnArgs& a, const CUtensorMap& t
           const float p0 = exp2_approx(s[n]), p1 = exp2_approx(s[n + 1]);
           sum[n] = fmaf(p0, sc.y, sum[n]);
           sum[n + 1] = fmaf(p1, sc.y, sum[n + 1]);
-          const __half2 up = __float2half2_rn(32.f);
           const __half2 h = __floats2half2_rn(p0, p1);
-          const uint16_t ta = e4m3x2_from_f16x2(h);
-          const __half2 r1 = __hmul2(__hsub2(h, half2_from_e4m3x2(ta)), up);  // exact
-          const uint16_t tb = e4m3x2_from_f16x2(r1);
-          const uint16_t tc = e4m3x2_from_f16x2(__hmul2(__hsub2(r1, half2_from_e4m3x2(tb)), up));
+          const uint16_t ta = e5m2x2_from_f16x2(h);
+          // remainders: exact, at most 2^-3 and 2^-4 of the power of two below their term, so scaled they stay in range
+          const __half2 r1 = __hmul2(__hsub2(h, half2_from_e5m2x2(ta)), __float2half2_rn(8.f));
+          const uint16_t tb = e5m2x2_from_f16x2(r1);
+          const uint16_t tc = e5m2x2_from_f16x2(__hmul2(__hsub2(r1, half2_from_e5m2x2(tb)), __float2half2_rn(32.f)));
           const int k = i >> 1;
           if ((i & 1) == 0) w[0][k] = ta, w[1][k] = tb, w[2][k] = tc;
           else w[0][k] |= static_cast<uint32_t>(ta) << 16, w[1][k] |= static_cast<uint32_t>(tb) << 16, w[2][k] |= static_cast<uint32_t>(tc) << 16;
@@ -499,7 +505,7 @@ __device__ __forceinline__ void run(const PagedAttnArgs& a, const CUtensorMap& t
         float x[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          x[i] = (__uint_as_float(v[0][i]) + (__uint_as_float(v[1][i]) + __uint_as_float(v[2][i]) * 0.03125f) * 0.03125f) *
+          x[i] = (__uint_as_float(v[0][i]) + (__uint_as_float(v[1][i]) + __uint_as_float(v[2][i]) * 0.03125f) * 0.125f) *
                  b.factor[col0 + c * 8 + i];
         const int n0 = col0 + c * 8;
         if (it.splits == 1) {
