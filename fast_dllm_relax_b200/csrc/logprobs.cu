@@ -1,13 +1,20 @@
 // Log probabilities of given tokens, with entropy and top alternatives, from logits (fdllm_logprobs);
 // the reference reduces logits on the host (runners.py:877-881).  Per row of x, in fp32, with L = log2 e:
 //   M = max x,  S0 = sum 2^((x - M) L),  S1 = sum 2^((x - M) L) (x - M) L
-//   lse = M + ln S0,  logprob = x[target] - lse,  entropy = ln S0 - ln 2 S1 / S0
-// and the `top` largest by (value descending, id ascending).
+//   logprob = (x[target] - M) - ln S0,  entropy = ln S0 - ln 2 S1 / S0
+// and the `top` largest by (value descending, id ascending).  S0 >= 1 and S1 <= 0, so a log probability is never
+// positive and an entropy never negative.
 //
 // Bound: HBM, every logit read once.  A row is split into parts of whole chunks (256 threads x four
-// 16-byte granules), a CTA a part.  A thread keeps its own running (M, S0, S1) and the next chunk's
-// granules in flight, so the main loop has no barrier:
-//   - moving (M, S0, S1) to another maximum N: d = (M - N) L, f = 2^d, S1' = f (S1 + S0 d), S0' = f S0;
+// 16-byte granules), a CTA a part.  A thread keeps its own running (B, S0, S1) relative to a base B, its maximum and the
+// next chunk's granules in flight, so the main loop has no barrier:
+//   - moving (B, S0, S1) to another base N: d = (B - N) L, f = 2^d, S1' = f (S1 + S0 d), S0' = f S0.  B starts at
+//     the maximum of the part's first chunk and follows the thread's only when that is kLag above it, which few
+//     chunks see; at the end all move to the row's maximum.  S1 + S0 d cancels what the lag put into S1, to 2^-24 of
+//     lag S0; but a base lags only where another logit is within kLag of the maximum, so where the entropy is a good
+//     part of a nat.  A peak that stands alone is its thread's base: its terms are exactly 1 and 0, and S0 keeps what
+//     its additions round away beside that 1 (a lag of 40 and no such sum took 106 us for
+//     the 108 below, and gave a peaked row's entropy 4e-6 to 2e-5 off);
 //   - the alternatives without sorting: in the part's first chunk the `top`-th largest of the 64 maxima
 //     of 4-thread groups is a lower bound of its `top`-th largest logit.  Later logits matter only when
 //     they exceed that bound (at equality the earlier ids win), so a chunk costs one compare a thread, and
@@ -17,7 +24,7 @@
 // The last CTA of a row (an arrival counter) joins the parts' statistics in part order and merges their
 // sorted lists, so one launch serves any split and the result does not depend on the arrival order.
 //
-// Measured, fp32, 151936 logits a row, five alternatives: 1024 rows 107 us, 5.8 TB/s; 256 rows 36.2 us, 4.3 TB/s (512
+// Measured, fp32, 151936 logits a row, five alternatives: 1024 rows 108 us, 5.8 TB/s; 256 rows 36.2 us, 4.3 TB/s (512
 // CTAs, one wave); one row 9.3 us (38 CTAs: latency of a chunk, its ranking and the join).
 #include <algorithm>
 
@@ -32,6 +39,7 @@ constexpr int kNV = 4;             // granules a thread per chunk
 constexpr int kGroups = 64;        // 4-thread groups whose maxima bound the alternatives
 constexpr int kMaxCand = 512;      // candidates of a part that are ranked by counting
 constexpr int kMaxParts = 64;      // of a row: the last CTA holds their lists in shared memory
+constexpr float kLag = 2.f;        // nats that a thread's maximum may be above its base
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 static_assert(kMaxTopLogprobs <= kGroups, "the bound needs `top` groups");
@@ -147,7 +155,7 @@ struct Row {
   }
 };
 
-__device__ __forceinline__ void join(float& M, float& s0, float& s1, float N) {  // to the larger maximum N
+__device__ __forceinline__ void join(float& M, float& s0, float& s1, float N) {  // to the larger base N
   if (N == M || M == -INFINITY) {
     M = N;
     return;
@@ -168,20 +176,20 @@ __device__ __forceinline__ float target_logit(const LogprobArgs& a, int row) {
   return NAN;
 }
 
-// The results of a row from its joined statistics and merged alternatives (lane < top holds one);
+// The results of a row from its statistics, joined at its maximum M, and merged alternatives (lane < top holds one);
 // xt: the target's logit, in lane 0.
 __device__ __forceinline__ void write_row(const LogprobArgs& a, int row, float M, float s0, float s1, float xt, Key key,
                                           int lane) {
   // no distribution: only -inf logits (S0 = 0), or a NaN or +inf one (S0 = NaN)
-  const float ls = s0 > 0.f ? logf(s0) : NAN;
-  const float lse = M + ls;
+  // the maximum's own term is 1, and no term of S1 is positive: what is below or above is rounding
+  const float ls = s0 > 0.f ? logf(fmaxf(s0, 1.f)) : NAN;
   if (lane == 0) {
-    if (a.targets != nullptr) a.logprob[row] = xt - lse;
-    if (a.entropy != nullptr) a.entropy[row] = ls - kLn2 * (s1 / s0);
+    if (a.targets != nullptr) a.logprob[row] = (xt - M) - ls;
+    if (a.entropy != nullptr) a.entropy[row] = ls - kLn2 * (fminf(s1, 0.f) / s0);
   }
   if (lane < a.top) {
     a.top_ids[static_cast<size_t>(row) * a.top + lane] = static_cast<int>(~static_cast<uint32_t>(key));
-    a.top_logprobs[static_cast<size_t>(row) * a.top + lane] = value_of(static_cast<uint32_t>(key >> 32)) - lse;
+    a.top_logprobs[static_cast<size_t>(row) * a.top + lane] = (value_of(static_cast<uint32_t>(key >> 32)) - M) - ls;
   }
 }
 
@@ -265,7 +273,7 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_kernel(const LogprobArgs
   __shared__ float s_M[8], s_s0[8], s_s1[8];
   __shared__ Key s_cand[kMaxCand], s_top[kMaxTopLogprobs], s_best[8];
   extern __shared__ Key s_lists[];  // [parts * top], the last CTA's merge
-  __shared__ float s_tau;
+  __shared__ float s_tau, s_base;
   __shared__ int s_count, s_last;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int r = blockIdx.x / parts, part = blockIdx.x % parts;
@@ -280,7 +288,8 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_kernel(const LogprobArgs
   const int chunks = static_cast<int>((static_cast<long long>(a.vocab) + row.off + kThreads * E - 1) / (kThreads * E));
   const int c0 = part * part_chunks, c1 = min(c0 + part_chunks, chunks);
 
-  float M = -INFINITY, s0 = 0.f, s1 = 0.f, bound = -INFINITY;
+  float M = -INFINITY, top_x = -INFINITY, s0 = 0.f, s1 = 0.f, bound = -INFINITY;  // M: the base, top_x: the maximum
+  float lost = 0.f;  // what the additions to S0 rounded away: beside a peak's 1 a chunk's terms may be below half a unit
   uint4 next[kNV];
   row.load(c0, next);
   for (int c = c0; c < c1; ++c) {
@@ -294,28 +303,31 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_kernel(const LogprobArgs
       gmax[j] = Vec<T>::largest(cur[j]);
       cm = fmaxf(cm, gmax[j]);
     }
-    if (a.top > 0) {
-      if (c == c0) {
-        float gm = fmaxf(cm, __shfl_xor_sync(0xffffffffu, cm, 1));
-        gm = fmaxf(gm, __shfl_xor_sync(0xffffffffu, gm, 2));
-        if ((lane & 3) == 0) s_group[threadIdx.x >> 2] = rank_of(gm);
-        __syncthreads();
-        {  // the `top`-th largest group maximum: four threads count a group's rank, a quarter each
-          const int g = threadIdx.x >> 2, o0 = (lane & 3) * (kGroups / 4);
-          const uint32_t mine = s_group[g];
-          int rank = 0;
+    top_x = fmaxf(top_x, cm);
+    if (c == c0) {
+      float gm = fmaxf(cm, __shfl_xor_sync(0xffffffffu, cm, 1));
+      gm = fmaxf(gm, __shfl_xor_sync(0xffffffffu, gm, 2));
+      if ((lane & 3) == 0) s_group[threadIdx.x >> 2] = rank_of(gm);
+      __syncthreads();
+      {  // the largest and the `top`-th largest group maximum: four threads count a group's rank, a quarter each
+        const int g = threadIdx.x >> 2, o0 = (lane & 3) * (kGroups / 4);
+        const uint32_t mine = s_group[g];
+        int rank = 0;
 #pragma unroll
-          for (int o = 0; o < kGroups / 4; ++o) {
-            const uint32_t other = s_group[o0 + o];
-            rank += other > mine || (other == mine && o0 + o < g);
-          }
-          rank += __shfl_xor_sync(0xffffffffu, rank, 1);
-          rank += __shfl_xor_sync(0xffffffffu, rank, 2);
-          if (rank == a.top - 1) s_tau = value_of(mine);
+        for (int o = 0; o < kGroups / 4; ++o) {
+          const uint32_t other = s_group[o0 + o];
+          rank += other > mine || (other == mine && o0 + o < g);
         }
-        __syncthreads();
-        bound = s_tau;
+        rank += __shfl_xor_sync(0xffffffffu, rank, 1);
+        rank += __shfl_xor_sync(0xffffffffu, rank, 2);
+        if (rank == 0) s_base = value_of(mine);
+        if (rank == a.top - 1) s_tau = value_of(mine);
       }
+      __syncthreads();
+      M = s_base;
+      if (a.top > 0) bound = s_tau;
+    }
+    if (a.top > 0) {
       // logits that reach the bound; a NaN passes (the comparison is negated) and ranks as -inf
 #pragma unroll
       for (int j = 0; j < kNV; ++j) {
@@ -352,10 +364,12 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_kernel(const LogprobArgs
         __syncthreads();
       }
     }
-    // the base moves only when the maximum outgrows it by 2^57: sums stay far from overflow, and a base
-    // below the maximum costs no precision
-    if (cm > M + 40.f) join(M, s0, s1, cm);
+    if (cm > M + kLag) {
+      s0 += lost, lost = 0.f;
+      join(M, s0, s1, cm);
+    }
     const float base = M == -INFINITY ? 0.f : M;
+    float sum = 0.f;
 #pragma unroll
     for (int j = 0; j < kNV; ++j) {
       float v[V];
@@ -363,14 +377,18 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_kernel(const LogprobArgs
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         const float d = (v[i] - base) * kLog2e, e = exp2_approx(d);
-        s0 += e;
+        sum += e;
         s1 = fmaf(e, fmaxf(d, -1e30f), s1);  // a logit of -inf adds 0, not 0 * inf
       }
     }
+    const float both = s0 + sum;
+    lost += sum - (both - s0);  // exact where S0 is the larger, as it is from a peak on
+    s0 = both;
   }
+  s0 += lost;
 
   // the part's statistics: the block's maximum, then the threads' sums relative to it
-  float W = warp_max(M);
+  float W = warp_max(top_x);
   if (lane == 0) s_M[warp] = W;
   __syncthreads();  // also: every candidate is in the buffer
   W = s_M[0];
