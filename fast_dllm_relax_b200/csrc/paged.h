@@ -216,7 +216,9 @@ __device__ __forceinline__ void paged_stage_queries(const PagedAttnArgs& a, cons
     uint32_t m = max(m2 & 0xFFFFu, m2 >> 16);
 #pragma unroll
     for (int d = kLanes / 2; d > 0; d >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
-    // exponent of the maximum (a bf16's bits), kept where both the scale and its inverse are normal floats
+    // exponent of the maximum (a bf16's bits), kept where both the scale and its inverse are normal floats; a row that
+    // is not finite has no weights: its scores become NaN below (the codes saturate)
+    const bool finite = m < 0x7F80u;
     int e = min(max(static_cast<int>(m >> 7) - 127, -110), 110);
     if (m == 0u) e = 7;
     const float up = __uint_as_float(static_cast<uint32_t>(127 + 7 - e) << 23);
@@ -240,7 +242,7 @@ __device__ __forceinline__ void paged_stage_queries(const PagedAttnArgs& a, cons
       }
     }
     if (part == 0) {
-      rows.unscale[n] = a.scale * kLog2e * __uint_as_float(static_cast<uint32_t>(127 + e - 7) << 23);
+      rows.unscale[n] = finite ? a.scale * kLog2e * __uint_as_float(static_cast<uint32_t>(127 + e - 7) << 23) : NAN;
       rows.out[n] = (it.tok0 + t) * a.hq + h;
       rows.lim[n] = n < it.rows ? min(it.key1, paged_key_limit(it.len, it.start + t, a.causal_block)) : it.key1;
     }

@@ -141,14 +141,14 @@ __global__ void __launch_bounds__(32 * kWarps, 2) paged_attn_simt_kernel(const P
     float mx = sm[0][h];
 #pragma unroll
     for (int w = 1; w < kWarps; ++w) mx = fmaxf(mx, sm[w][h]);
-    float num = 0.f, den = 0.f;
+    float num = 0.f, den = 0.f;  // den: 0 without keys, NaN where a score is not a number
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
       const float f = sm[w][h] == -INFINITY ? 0.f : exp2f(sm[w][h] - mx);
       num += f * so[w][h][d];
       den += f * sl[w][h];
     }
-    static_cast<float*>(a.out)[(static_cast<size_t>(tok) * a.hq + head0 + h) * HD + d] = den > 0.f ? num / den : 0.f;
+    static_cast<float*>(a.out)[(static_cast<size_t>(tok) * a.hq + head0 + h) * HD + d] = den == 0.f ? 0.f : num / den;
   }
 }
 

@@ -185,13 +185,14 @@ __device__ __forceinline__ void run(const PagedAttnArgs& a, const CUtensorMap& t
       for (int j = 0; j < HD / 32; ++j) m = fmaxf(m, fabsf(x[k][j]));
 #pragma unroll
       for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-      // exponent of m, kept where both the scale and its inverse are normal floats
+      // exponent of m, kept where both the scale and its inverse are normal floats; an infinite row has no weights
       int e = min(max(static_cast<int>(__float_as_uint(m) >> 23) - 127, -110), 110);
       if (m == 0.f) e = 7;
       const float up = __uint_as_float(static_cast<uint32_t>(127 + 7 - e) << 23);
 #pragma unroll
       for (int j = 0; j < HD / 32; ++j) sq[i * (HD + 8) + lane + 32 * j] = __float2half_rn(x[k][j] * up);
-      if (lane == 0) s_unscale[i] = a.scale * kLog2e * __uint_as_float(static_cast<uint32_t>(127 + e - 7) << 23);
+      if (lane == 0)
+        s_unscale[i] = m < INFINITY ? a.scale * kLog2e * __uint_as_float(static_cast<uint32_t>(127 + e - 7) << 23) : NAN;
     }
     named_sync(1, 32 * kWarps);
     uint32_t qf[KS][NT][2];  // B fragments: columns are query rows, the reduction order is the K fragment's
