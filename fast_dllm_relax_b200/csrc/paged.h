@@ -219,7 +219,7 @@ __device__ __forceinline__ void paged_stage_queries(const PagedAttnArgs& a, cons
     // exponent of the maximum (a bf16's bits), kept where both the scale and its inverse are normal floats; a row that
     // is not finite has no weights: its scores become NaN below (the codes saturate)
     const bool finite = m < 0x7F80u;
-    int e = min(max(static_cast<int>(m >> 7) - 127, -110), 110);
+    int e = max(static_cast<int>(m >> 7) - 127, -110);
     if (m == 0u) e = 7;
     const float up = __uint_as_float(static_cast<uint32_t>(127 + 7 - e) << 23);
     if (kPad || n < it.rows) {

@@ -186,7 +186,7 @@ __device__ __forceinline__ void run(const PagedAttnArgs& a, const CUtensorMap& t
 #pragma unroll
       for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
       // exponent of m, kept where both the scale and its inverse are normal floats; an infinite row has no weights
-      int e = min(max(static_cast<int>(__float_as_uint(m) >> 23) - 127, -110), 110);
+      int e = max(static_cast<int>(__float_as_uint(m) >> 23) - 127, -110);
       if (m == 0.f) e = 7;
       const float up = __uint_as_float(static_cast<uint32_t>(127 + 7 - e) << 23);
 #pragma unroll
