@@ -484,7 +484,8 @@ __device__ __forceinline__ void run(const PagedAttnArgs& a, const CUtensorMap& t
     named_sync(2, 256);
     const int t = threadIdx.x - 128;
     if (t < N) {
-      const float l = b.part[0][t] + b.part[1][t] + b.part[2][t] + b.part[3][t];
+      float l = b.part[0][t] + b.part[1][t] + b.part[2][t] + b.part[3][t];
+      if (l == INFINITY) l = NAN;  // a score past fp32: P's terms saturate, the quotient must not pass for a result
       b.factor[t] = it.splits == 1 ? (l != 0.f ? 1.f / l : 0.f) : 1.f;
       b.delta[t] = l;
     }
