@@ -8,7 +8,8 @@
 //   code = e4m3(value / s),  kept codes = e4m3(code_old * s_old / s)
 //
 // A power of two makes both divisions exact, so a value is rounded once, and a kept code only loses
-// bits where it becomes subnormal.
+// bits where it becomes subnormal.  A page that keeps a larger scale of its own, which need not be one (a cache that
+// another program filled), takes the rounded quotients.
 //
 // Bound: HBM (every input read once, every output written once).  One launch, two kinds of CTAs:
 //   - a page, KV head and K or V: a thread holds up to two 8-column chunk pairs (K) or four chunks (V) of the
@@ -75,6 +76,19 @@ __device__ __forceinline__ void rotate8(float (&x)[8], float (&y)[8], const floa
     y[i] = y[i] * c[i] + x[i] * s[i];
     x[i] = a;
   }
+}
+
+// 1 / s for a power of two; for another scale 1, and the values become their quotients here: by the inverse in 64 bits,
+// whose 2^-53 leaves a quotient of few bits, as one half way between two codes is, as it is.
+template <int N>
+__device__ __forceinline__ float inverse_scale(float s, float (&x)[N][8]) {
+  if ((__float_as_uint(s) & 0x7FFFFFu) == 0) return 1.f / s;
+  const double inv = 1.0 / s;
+#pragma unroll
+  for (int j = 0; j < N; ++j)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[j][i] = static_cast<float>(x[j][i] * inv);
+  return 1.f;
 }
 
 __device__ __forceinline__ uint2 code8(const float (&x)[8], float inv) {
@@ -172,7 +186,7 @@ __global__ void __launch_bounds__(512, 2) paged_append_kernel(const PagedAppendA
 #pragma unroll
         for (int e = 0; e < 8; ++e) amax = fmaxf(amax, finite_abs(x[j][e]));
     s = page_scale(amax, keeps, s_old, red);
-    const float inv = 1.f / s;
+    const float inv = inverse_scale(s, x);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int i = tid + j * blockDim.x;
@@ -204,7 +218,8 @@ __global__ void __launch_bounds__(512, 2) paged_append_kernel(const PagedAppendA
       }
     }
     s = page_scale(amax, keeps, s_old, red);
-    const float inv = 1.f / s;
+    const float inv = inverse_scale(s, x);
+    (void)inverse_scale(s, y);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const int i = tid + j * blockDim.x;
