@@ -187,7 +187,22 @@ def generate_batch(engine: Engine, prompts: Sequence[Sequence[int]], *, max_new_
     """Decode every prompt; returns (continuations, per-request statistics).  `timing`, when a
     dict, receives total_ms and prefill_ms (the prefix-cache builds), measured with CUDA events.
     `pool`: keep the requests' keys and values in its paged 8-bit cache (fdllm_forward_paged) instead of one
-    bf16 cache a request; its pages come back when a request is done."""
+    bf16 cache a request; its pages come back when a request is done, and all of them when the call ends in an
+    error."""
+    held: dict[int, list] = {}  # page lists of the requests
+    try:
+        return _generate_batch(engine, prompts, max_new_tokens=max_new_tokens, block_size=block_size,
+                               small_block_size=small_block_size, threshold=threshold, use_block_cache=use_block_cache,
+                               mask_id=mask_id, stop_token=stop_token, timing=timing, pool=pool, held=held)
+    finally:
+        for pages in itertools.chain.from_iterable(held.values()):
+            pool.release(pages)
+
+
+def _generate_batch(engine: Engine, prompts: Sequence[Sequence[int]], *, max_new_tokens: int, block_size: int,
+                    small_block_size: int, threshold: float, use_block_cache: bool, mask_id: int,
+                    stop_token: int | None, timing: dict | None, pool: PagedPool | None,
+                    held: dict[int, list]) -> tuple[list[list[int]], list[dict]]:
     if block_size != engine.cfg.bd_size:
         raise ValueError("block_size must equal the model's bd_size")
     dev = engine.device
@@ -207,8 +222,6 @@ def generate_batch(engine: Engine, prompts: Sequence[Sequence[int]], *, max_new_
             pending.pop(i, None)
             for pages in held.pop(i, ()):
                 pool.release(pages)
-
-    held: dict[int, list] = {}  # page lists of the requests (a pool's pages go back when one is done)
 
     def paged_forward(ops, x, rows, start, live, causal_block, hidden):
         """One forward of several requests over the pool's cache, their pages extended first."""

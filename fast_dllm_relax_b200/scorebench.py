@@ -48,21 +48,23 @@ def score_batch(eng: Engine, caches, ctx: torch.Tensor, blocks: torch.Tensor, ta
 def score_batch_paged(eng: Engine, pool: PagedPool, ctx: torch.Tensor, blocks: torch.Tensor, targets: torch.Tensor,
                       n_cont: int, top: int):
     """score_batch over a paged 8-bit cache: (sums [b], entropies [b, n_cont], alternatives' ids and log
-    probabilities [b, n_cont, top]).  The contexts' pages go back to the pool."""
+    probabilities [b, n_cont, top]).  The contexts' pages go back to the pool, after an error too."""
     b, C = ctx.shape
     rows = blocks.shape[1]
     pages: list[list[int]] = [[] for _ in range(b)]
-    for p in pages:
-        pool.grow(p, C + rows)
-    table, ps = pool.table(pages), pool.cache.page_size
-    plan = eng.paged_plan([C] * b, [0] * b, page_size=ps, causal_block=eng.cfg.bd_size)
-    eng.forward_paged(eng.embed(ctx.reshape(-1)), pool.cache, plan, table, hidden=False)
-    plan = eng.paged_plan([rows] * b, [C] * b, page_size=ps)
-    hidden = eng.forward_paged(eng.embed(blocks.reshape(-1)), pool.cache, plan, table)
-    hidden = hidden.view(b, rows, -1)[:, :n_cont].reshape(b * n_cont, -1)
-    lp, ent, ids, tlp = eng.logprobs(eng.get_logits(hidden), targets[:, :n_cont].reshape(-1), top=top)
-    for p in pages:
-        pool.release(p)
+    try:
+        for p in pages:
+            pool.grow(p, C + rows)
+        table, ps = pool.table(pages), pool.cache.page_size
+        plan = eng.paged_plan([C] * b, [0] * b, page_size=ps, causal_block=eng.cfg.bd_size)
+        eng.forward_paged(eng.embed(ctx.reshape(-1)), pool.cache, plan, table, hidden=False)
+        plan = eng.paged_plan([rows] * b, [C] * b, page_size=ps)
+        hidden = eng.forward_paged(eng.embed(blocks.reshape(-1)), pool.cache, plan, table)
+        hidden = hidden.view(b, rows, -1)[:, :n_cont].reshape(b * n_cont, -1)
+        lp, ent, ids, tlp = eng.logprobs(eng.get_logits(hidden), targets[:, :n_cont].reshape(-1), top=top)
+    finally:
+        for p in pages:
+            pool.release(p)
     return lp.view(b, n_cont).sum(dim=1), ent.view(b, n_cont), ids.view(b, n_cont, top), tlp.view(b, n_cont, top)
 
 
