@@ -336,8 +336,11 @@ class Engine:
         n = len(rows)
         if len(start) != n or (live is not None and len(live) != n):
             raise ValueError("paged_plan: one start (and live) per request")
-        arrays = [(ctypes.c_int32 * max(n, 1))(*[int(x) for x in a]) if a is not None else None
-                  for a in (rows, start, live)]
+        lists = [[int(x) for x in a] if a is not None else None for a in (rows, start, live)]
+        for values in (*lists, [int(page_size), int(causal_block)]):  # ctypes would keep the low 32 bits
+            if values and not (min(values) >= -2 ** 31 and max(values) < 2 ** 31):
+                raise ValueError("paged_plan: rows, positions and blocks must fit 32 bits")
+        arrays = [(ctypes.c_int32 * max(n, 1))(*a) if a is not None else None for a in lists]
         desc = _lib.FdllmPagedPlan()
         args = (self._h, *arrays, n, int(page_size), int(causal_block))
         _lib.check(self.lib.fdllm_paged_plan_batch(*args, None, 0, ctypes.byref(desc)))
