@@ -500,7 +500,7 @@ class Engine:
                              f"{tuple(t.shape)} on {t.device}")
         ld, one = t.stride()
         if one != 1 or ld < cols or (ld * self._esz | t.data_ptr()) & 15:
-            t = t.contiguous() if not t.is_contiguous() else t.clone()
+            t = t.new_empty((rows, cols)).copy_(t)  # (contiguous() and clone() keep a lone row's stride)
         return t
 
     def _raw_stream(self) -> int:
