@@ -6,15 +6,15 @@
 // positive and an entropy never negative.
 //
 // Bound: HBM, every logit read once.  A row is split into parts of whole chunks (256 threads x four
-// 16-byte granules), a CTA a part.  A thread keeps its own running (B, S0, S1) relative to a base B, its maximum and the
-// next chunk's granules in flight, so the main loop has no barrier:
+// 16-byte granules), a CTA a part.  A thread keeps its own running (B, S0, S1) relative to a base B, its maximum and
+// the next chunk's granules in flight, so the main loop has no barrier:
 //   - moving (B, S0, S1) to another base N: d = (B - N) L, f = 2^d, S1' = f (S1 + S0 d), S0' = f S0.  B starts at
 //     the maximum of the part's first chunk and follows the thread's only when that is kLag above it, which few
 //     chunks see; at the end all move to the row's maximum.  S1 + S0 d cancels what the lag put into S1, to 2^-24 of
 //     lag S0; but a base lags only where another logit is within kLag of the maximum, so where the entropy is a good
-//     part of a nat.  A peak that stands alone is its thread's base: its terms are exactly 1 and 0, and S0 keeps what
-//     its additions round away beside that 1 (a lag of 40 and no such sum took 106 us for
-//     the 108 below, and gave a peaked row's entropy 4e-6 to 2e-5 off);
+//     part of a nat.  A peak that stands alone is its thread's base: its terms are exactly 1 and 0, and the chunks
+//     after it are summed apart, as their terms may be below half a unit of that 1 (a base up to 40 behind and one
+//     sum took 107.5 us for the 109 below, and gave a peaked row's entropy 4e-6 to 2e-5 off);
 //   - the alternatives without sorting: in the part's first chunk the `top`-th largest of the 64 maxima
 //     of 4-thread groups is a lower bound of its `top`-th largest logit.  Later logits matter only when
 //     they exceed that bound (at equality the earlier ids win), so a chunk costs one compare a thread, and
@@ -24,8 +24,8 @@
 // The last CTA of a row (an arrival counter) joins the parts' statistics in part order and merges their
 // sorted lists, so one launch serves any split and the result does not depend on the arrival order.
 //
-// Measured, fp32, 151936 logits a row, five alternatives: 1024 rows 108 us, 5.8 TB/s; 256 rows 36.2 us, 4.3 TB/s (512
-// CTAs, one wave); one row 9.3 us (38 CTAs: latency of a chunk, its ranking and the join).
+// Measured, fp32, 151936 logits a row, five alternatives: 1024 rows 109 us, 5.7 TB/s; 256 rows 36.8 us, 4.2 TB/s (512
+// CTAs, one wave); one row 9.6 us (38 CTAs: latency of a chunk, its ranking and the join).
 #include <algorithm>
 
 #include "paged.h"
@@ -289,7 +289,7 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_kernel(const LogprobArgs
   const int c0 = part * part_chunks, c1 = min(c0 + part_chunks, chunks);
 
   float M = -INFINITY, top_x = -INFINITY, s0 = 0.f, s1 = 0.f, bound = -INFINITY;  // M: the base, top_x: the maximum
-  float lost = 0.f;  // what the additions to S0 rounded away: beside a peak's 1 a chunk's terms may be below half a unit
+  float rest = 0.f;  // of S0, the chunks since the one that set the base
   uint4 next[kNV];
   row.load(c0, next);
   for (int c = c0; c < c1; ++c) {
@@ -364,8 +364,9 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_kernel(const LogprobArgs
         __syncthreads();
       }
     }
-    if (cm > M + kLag) {
-      s0 += lost, lost = 0.f;
+    const bool peak = cm > M + kLag;
+    if (peak) {
+      s0 += rest, rest = 0.f;
       join(M, s0, s1, cm);
     }
     const float base = M == -INFINITY ? 0.f : M;
@@ -381,11 +382,10 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_kernel(const LogprobArgs
         s1 = fmaf(e, fmaxf(d, -1e30f), s1);  // a logit of -inf adds 0, not 0 * inf
       }
     }
-    const float both = s0 + sum;
-    lost += sum - (both - s0);  // exact where S0 is the larger, as it is from a peak on
-    s0 = both;
+    if (peak || c == c0) s0 += sum;
+    else rest += sum;
   }
-  s0 += lost;
+  s0 += rest;
 
   // the part's statistics: the block's maximum, then the threads' sums relative to it
   float W = warp_max(top_x);
