@@ -14,7 +14,7 @@
 //     lag S0; but a base lags only where another logit is within kLag of the maximum, so where the entropy is a good
 //     part of a nat.  A peak that stands alone is its thread's base: its terms are exactly 1 and 0, and the chunks
 //     after it are summed apart, as their terms may be below half a unit of that 1 (a base up to 40 behind and one
-//     sum took 107.5 us for the 109 below, and gave a peaked row's entropy 4e-6 to 2e-5 off);
+//     sum took 107.5 us where this takes 108.9, and gave a peaked row's entropy 4e-6 to 2e-5 off);
 //   - the alternatives without sorting: in the part's first chunk the `top`-th largest of the 64 maxima
 //     of 4-thread groups is a lower bound of its `top`-th largest logit.  Later logits matter only when
 //     they exceed that bound (at equality the earlier ids win), so a chunk costs one compare a thread, and
@@ -24,7 +24,7 @@
 // The last CTA of a row (an arrival counter) joins the parts' statistics in part order and merges their
 // sorted lists, so one launch serves any split and the result does not depend on the arrival order.
 //
-// Measured, fp32, 151936 logits a row, five alternatives: 1024 rows 109 us, 5.7 TB/s; 256 rows 36.8 us, 4.2 TB/s (512
+// Measured, fp32, 151936 logits a row, five alternatives: 1024 rows 106 to 109 us, 5.8 TB/s; 256 rows 36.8 us, 4.2 TB/s (512
 // CTAs, one wave); one row 9.6 us (38 CTAs: latency of a chunk, its ranking and the join).
 #include <algorithm>
 

@@ -8,7 +8,7 @@
 //   s_t = scale (q . k_t),  o = o 2^(m - m') + sum_t 2^(s_t - m') v_t   (base-2 exponents, fp32)
 // with the 32 value rows' loads in flight together.  The warps' (m, l, o) are joined through shared memory.
 // Bound by latency at the sizes it serves (parity checks): 4 requests of 8 to 32 rows over 65 to 515 keys, 4/2 heads of
-// 64, take 10.3 us (a CTA of four warps a query head: 16.5), 3 of 32 rows over up to 609 keys, 12/2 heads of 128, 22.4
+// 64, take 10.3 us (a CTA of four warps a query head: 16.5), 3 of 32 rows over up to 609 keys, 12/2 heads of 128, 21.7
 // (34.2).
 #include "paged.h"
 

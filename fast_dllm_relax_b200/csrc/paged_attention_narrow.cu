@@ -23,7 +23,7 @@
 // A tile whose keys are split over several items joins them through the workspace: the last item to arrive
 // (a counter) adds the partials in item order, so the result does not depend on the arrival order.
 //
-// Measured, 8/8 heads of 64: 64 tokens over 1000 keys each 21.5 us, 3.1 TB/s (latency: 512 CTAs of eight stages, a
+// Measured, 8/8 heads of 64: 64 tokens over 1000 keys each 21.2 us, 3.1 TB/s (latency: 512 CTAs of eight stages, a
 // chain of item, page ids, scales and copies before the first); 56 prompts of 5 to 734 rows 74 us, where the 3000
 // tiles' prologues and joins take more than their products.
 #include "paged.h"

@@ -32,8 +32,8 @@
 // partials in item order (paged_join).
 //
 // Measured, 12/2 heads of 128: one token over 397 keys 8.3 us (a chain of latencies: item, page ids, scales, copies,
-// two products, the join), over 32000 keys 16.7; 64 tokens over 700 to 8191 keys 24.8 us, 4.1 TB/s (102 MB: each of
-// the 284 items waits through its prologue once, and they end unevenly); 8 rows of 8 requests over 4096 keys 19.8 us.
+// two products, the join), over 32000 keys 16.7; 64 tokens over 700 to 8191 keys 24.9 us, 4.1 TB/s (102 MB: each of
+// the 284 items waits through its prologue once, and they end unevenly); 8 rows of 8 requests over 4096 keys 19.6 us.
 #pragma once
 #include "paged_mma.cuh"
 

@@ -20,14 +20,14 @@
 // CTAs share an SM (256 TMEM columns and 110 KB each), so one's softmax covers the other's products.
 //
 // Measured, 12/2 heads of 128: 2 prompts of 4096 tokens, block-causal, 123 us, 845 TFLOP/s of the formula's two
-// products; 32 block steps of 32 rows over 512 to 1024 keys 22.2 us, 8 over 4096 keys 28.7.
+// products; 32 block steps of 32 rows over 512 to 1024 keys 22.1 us, 8 over 4096 keys 27.9.
 //
-// What bounds it: no one pipe.  A tile of 8192 scores takes 950 clocks of an SM, of which the tensor core with its
-// operand reads is busy 62 % (Q is read twice for S, at 64 bytes a clock), the exponentials 42 % and issue 57 %; the
-// chain S, softmax, P, O of two CTAs does not keep any of them full, each wait on a barrier in it costs 100 clocks, and
-// 768 items' prologues and epilogues are a fifth of the prompts' time.  What did not shorten it, of 134 us then: S of
-// two tiles in one product (159), half a row a thread on eight softmax warps (134.5), one S and two P buffers (140),
-// that with Qh in TMEM (147).
+// What bounds it: no one pipe.  A tile of 8192 scores takes 1260 clocks of an SM (296 items, 1.28 us a key tile); over
+// the prompts the tensor core with its operand reads is busy 62 % (Q is read twice for S, at 64 bytes a clock), the
+// exponentials 42 % and issue 57 %.  The chain S, softmax, P, O of two CTAs does not keep any of them full, each wait on
+// a barrier in it costs 100 clocks, and launch, prologues and epilogues of 768 items, 27 us, are a fifth of the prompts'
+// time.  What did not shorten it, of 134 us then: S of two tiles in one product (159), half a row a thread on eight
+// softmax warps (134.5), one S and two P buffers (140), that with Qh in TMEM (147).
 //
 // A tile whose keys are split over several items joins them through the workspace: the last item to arrive adds the
 // partials in item order (paged_join).

@@ -241,7 +241,7 @@ FDLLM_API int fdllm_confidence_static(fdllm_handle* h, const void* hidden, int r
 typedef struct fdllm_paged_cache {
   void* k;               /* e4m3 codes [layers, pages, kv_heads, page_size, head_dim], 16-byte aligned */
   void* v;
-  float* k_scale;        /* fp32 [layers, pages, kv_heads], normal positive */
+  float* k_scale;        /* fp32 [layers, pages, kv_heads], normal positive (the append writes powers of two) */
   float* v_scale;
   int32_t layers;
   int32_t pages;
@@ -284,7 +284,7 @@ FDLLM_API int fdllm_paged_plan_batch(fdllm_handle* h, const int32_t* rows, const
  * no queries).  Rotated keys and the values are coded straight from fp32, one rounding:
  *   scale of a touched page = the least power of two (>= 2^-64) that brings its new finite values
  *   into +-448, or the page's present scale if that is larger and the page keeps rows;
- *   code = e4m3(value / scale), nearest even; infinities saturate, NaN stays NaN.
+ *   code = e4m3(value / scale), the fp32 quotient, nearest even; infinities saturate, NaN stays NaN.
  * Rows of a touched page below `live` and outside the written range keep their values; when the
  * scale grows their codes are rounded again to it (exact for e4m3 normal results).  Other rows of
  * the page are not read or written.  table: device int32 [n, table_ld] page ids; an id outside
@@ -299,9 +299,14 @@ FDLLM_API int fdllm_paged_append(fdllm_handle* h, const fdllm_paged_cache* cache
 /* Attention of the batch's token rows over the cache: q [total_rows, heads * head_dim] (rotated, row
  * stride ldq elements, 16-byte aligned rows) -> out [total_rows, heads * head_dim] (contiguous),
  *   out = sum_t softmax_t(scale * q . k_t) v_t   over the rows the plan's mask leaves,
- * fp32 softmax and accumulation; a token row that attends nothing gets zeros.  Cache rows at or past
- * a request's length are never used, whatever their bytes hold; rows below it must hold finite codes.
- * A page id outside [0, pages) is read as page 0 and records device error 6. */
+ * fp32 softmax statistics and accumulation; a token row that attends nothing gets zeros.  In bf16 the operands of the products are rounded: a weight times
+ * its page's value scale keeps 11 bits down to 2^-21 of the row's largest such product and fewer below, the last
+ * lost at 2^-32; at head_dim 128 query elements below 2^-10 of the row's largest are held to 2^-18 of it.
+ * A row with a query element that is not finite, or with a score above fp32's range, is NaN.
+ * Cache rows at or past a request's length are never used, whatever their bytes hold; rows below it must hold
+ * finite codes.  A page id outside [0, pages) is read as page 0 and records device error 6.
+ * A call with a larger batch than any before grows the handle's workspace (a device-wide wait): make one such call
+ * before capturing any, and capture a graph again that was made before the workspace moved. */
 FDLLM_API int fdllm_paged_attention(fdllm_handle* h, const fdllm_paged_cache* cache, int layer,
                                     const fdllm_paged_plan* plan, const int32_t* plan_words, const int32_t* table,
                                     int table_ld, const void* q, int ldq, float scale, void* out, void* stream);
@@ -322,8 +327,10 @@ FDLLM_API int fdllm_forward_paged(fdllm_handle* h, const fdllm_paged_cache* cach
  *   entropy[row] = lse - sum softmax * logits    (nats; ids at -inf contribute nothing)
  *   top_ids / top_logprobs [rows, top]           the `top` (0..32, <= vocab) largest logits in order,
  *                                                ties to the lowest id, and their log probabilities.
- * targets + logprob, entropy and top_* may be NULL.  A row with a NaN logit, a +inf logit or only
- * -inf logits has NaN log probabilities and entropy; its ids order NaN as -inf. */
+ * The sums are relative to the row's largest logit: no log probability is positive, no entropy negative, and both
+ * keep their bits where they are small.  targets + logprob, entropy and top_* may be NULL.  A row with a NaN logit, a
+ * +inf logit or only -inf logits has NaN log probabilities and entropy; its ids order NaN as -inf.  The workspace
+ * grows as fdllm_paged_attention's. */
 FDLLM_API int fdllm_logprobs(fdllm_handle* h, const void* logits, int logits_dtype, int rows, int vocab, long long ld,
                              const int32_t* targets, int top, float* logprob, float* entropy, int32_t* top_ids,
                              float* top_logprobs, void* stream);
