@@ -29,3 +29,18 @@ def test_scores_beyond_fp32_give_nan(length, heads, dtype):
         assert got[0, 0].isnan().all(), rows
         assert got[0, 1:].isfinite().all(), rows
     assert eng.device_error() == 0
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("heads", [(12, 2, 128), (4, 2, 64)], ids=str)
+def test_a_negative_scale_is_the_scale_of_negated_queries(heads, dtype):
+    hq, hkv, hd = heads
+    eng = engine(heads, dtype)
+    for rows, length in ((1, 700), (5, 130), (8, 700), (32, 300)):
+        gen = torch.Generator().manual_seed(rows)
+        table, pages = make_table([length], 32, gen)
+        cache, table = random_cache(eng, pages, 32, gen), table.cuda()
+        q = torch.randn(rows, hq * hd, generator=gen).to(eng.dtype).cuda()
+        plan = eng.paged_plan([rows], [length - rows])
+        assert torch.equal(eng.paged_attention(cache, 0, plan, table, q, scale=-0.2),
+                           eng.paged_attention(cache, 0, plan, table, -q, scale=0.2))
