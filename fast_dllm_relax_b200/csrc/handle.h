@@ -96,17 +96,18 @@ struct LayerW {
   const void* ln2 = nullptr;
 };
 
-// Bumped whenever any workspace buffer is reallocated: captured graphs recorded before a bump hold
+// Bumped whenever a workspace buffer that a graph may hold is reallocated: captured graphs recorded before a bump hold
 // stale pointers and are recaptured.
 extern std::atomic<unsigned long long> g_ws_generation;
 
-template <typename P>
+// kInGraphs: whether the library's graphs (decode.cu) may hold its address.
+template <typename P, bool kInGraphs = true>
 struct DevBuf {
   P* p = nullptr;
   size_t n = 0;  // elements
   int ensure(size_t want, bool zero = false) {
     if (want <= n) return FDLLM_OK;
-    g_ws_generation.fetch_add(1);
+    if (kInGraphs) g_ws_generation.fetch_add(1);
     if (p) cudaFree(p);
     p = nullptr;
     n = 0;
@@ -127,6 +128,9 @@ struct DevBuf {
   }
   size_t bytes() const { return n * sizeof(P); }
 };
+
+template <typename P>
+using CallBuf = DevBuf<P, false>;  // used by calls outside the decode loop alone
 
 struct ProfPair {
   cudaEvent_t e0 = nullptr, e1 = nullptr;
@@ -210,12 +214,12 @@ struct fdllm_handle {
   DevBuf<float> attn_part, attn_part_lse;  // tcgen05 key-split partials
   DevBuf<float> persist_part;               // persistent-GEMM split-K partial tiles
   DevBuf<unsigned> persist_ctr;             // persistent-GEMM per-tile split counters (zero between launches)
-  DevBuf<uint8_t> paged_qkv;                // forward_paged: a layer's projected rows before RoPE
-  DevBuf<float4> paged_part;                // paged attention: partials of tiles whose keys are split
-  DevBuf<unsigned> paged_ctr;               //   and their arrived items (zero between launches)
-  DevBuf<float4> logprob_part;              // log-probability partials of a row's parts
-  DevBuf<unsigned long long> logprob_keys;  //   and their alternatives
-  DevBuf<unsigned> logprob_ctr;             //   and its arrived parts (zero between launches)
+  fdllm::CallBuf<uint8_t> paged_qkv;                // forward_paged: a layer's projected rows before RoPE
+  fdllm::CallBuf<float4> paged_part;                // paged attention: partials of tiles whose keys are split
+  fdllm::CallBuf<unsigned> paged_ctr;               //   and their arrived items (zero between launches)
+  fdllm::CallBuf<float4> logprob_part;              // log-probability partials of a row's parts
+  fdllm::CallBuf<unsigned long long> logprob_keys;  //   and their alternatives
+  fdllm::CallBuf<unsigned> logprob_ctr;             //   and its arrived parts (zero between launches)
   // kernel trace (fdllm_kernel_trace_enable / _read): phase stamps of every projection and
   // attention launch issued outside stream capture while enabled, 8 per launch, and their kinds
   bool ktrace_on = false;

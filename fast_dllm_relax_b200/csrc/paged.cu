@@ -33,7 +33,7 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 
 // At least n arrival counters: zero when allocated (in the order of the call's stream), and again after
 // every launch that uses them.
-int ensure_counters(DevBuf<unsigned>* b, size_t n, cudaStream_t s) {
+int ensure_counters(CallBuf<unsigned>* b, size_t n, cudaStream_t s) {
   if (b->n >= n) return FDLLM_OK;
   FDLLM_TRY(b->ensure(n));
   CUDA_TRY(cudaMemsetAsync(b->p, 0, b->bytes(), s));
